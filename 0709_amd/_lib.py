@@ -8,6 +8,7 @@ that is not on a HIP device raises instead of computing elsewhere.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from pathlib import Path
@@ -25,6 +26,11 @@ ATLAS_EHIP_BASE = -1000
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
 DTYPE_F32 = 2
+
+CACHE_16BIT = 0
+CACHE_E4M3 = 1
+CACHE_INT8 = 2
+QUANT_COMMIT_MAX_ITEMS = 64
 
 MASK_NONE = 0
 MASK_TREE = 1
@@ -157,6 +163,16 @@ _SIGNATURES: dict[str, list] = {
         _vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp, _vp, _vp, _vp,
         ctypes.c_int, ctypes.c_double, ctypes.c_int, ctypes.c_double, _c_i64, _vp, _vp, _vp, _vp, _vp,
     ],
+    "atlas_paged_attn": [ctypes.c_char_p, _vp],
+    "atlas_kv_append_quantized": [
+        _VPP, _VPP, ctypes.c_int, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _VPP,
+        _VPP, _c_i64, ctypes.c_int, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, ctypes.c_int, _c_i64, _c_i64,
+        _c_i64, _c_i64, _vp,
+    ],
+    "atlas_kv_commit_quantized": [
+        _VPP, _VPP, ctypes.c_int, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+        ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, _c_i64, _c_i64, _c_i64, _vp,
+    ],
     "atlas_tree_spec_build": [
         _vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, _c_i64, ctypes.c_int32, _vp, _c_i64, _vp, _vp, _vp,
     ],
@@ -254,6 +270,17 @@ def require_device(*tensors: torch.Tensor | None, what: str) -> torch.device:
     if device is None:
         raise ValueError(f"{what}: no tensor given")
     return device
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which launches go to ``device`` (no cost where it is the
+    current one already)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
 
 
 # torch's current raw stream handle, without building a Stream object

@@ -1,0 +1,277 @@
+"""Paged attention from device-side metadata, with scored and 8-bit variants.
+
+``paged_attention`` takes the page-table arrays of FlashInfer's paged metadata
+(``qo_indptr``, ``kv_indptr``, ``kv_indices``, ``kv_last_page_len``) as device
+tensors and needs no plan: the kernel reads every request's lengths itself, so a
+call costs no host work per request, can be captured in a HIP graph and replayed
+with other lengths, page tables and inputs in the same buffers.
+
+For a request with n queries and L keys, query i stands at position L - n + i::
+
+    s = sm_scale * q . k
+    s = logits_soft_cap * tanh(s / logits_soft_cap)
+    s = s - alibi_slopes[head] * |position(q) - position(k)|
+
+and the output is the softmax of s over the keys the query sees, times V.  Over an
+8-bit cache (e4m3 or int8 codes, ``quantized_kv.py``) k and v are the codes times
+their block's scale.
+
+The calls it extends: the Drafter's decode
+(src/atlas_0709/flashinfer_paged/sglang_page_attention.py:171-209, which passes
+``logits_soft_cap``, ``k_scale`` and ``v_scale`` per layer) and the Target's verify
+(flashinfer_full_verify.py:953-985).
+"""
+
+from __future__ import annotations
+
+import math
+import struct
+
+import torch
+
+from . import _lib
+from .tree_attention import _host_lists
+
+# Packed query rows (query token * group + head of the group) of one workgroup, in
+# row tiles of 16.
+ROWS_ONE_TILE = 16
+ROWS_BLOCK = 64
+# Workgroups to aim for when the keys are split, and the least keys of a split.
+TARGET_WORKGROUPS = 1024
+MIN_SPLIT_KEYS = 256
+MAX_SPLITS = 256
+
+CACHE_CODES = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
+
+# atlas_paged_attn_t: 14 pointers, 15 int64, 14 int32, 2 floats
+_ARGS = struct.Struct("=14P15q14i2f".replace("P", "Q"))
+
+
+def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int) -> tuple[int, int, int, int]:
+    """(row tiles, row blocks, splits, keys per split) of a call.
+
+    Up to 16 packed rows take the one-tile kernel, more the four-tile one.  Keys
+    are split until about TARGET_WORKGROUPS workgroups are there, in splits of at
+    least MIN_SPLIT_KEYS; a request shorter than ``max_kv_len`` takes fewer
+    splits of the same size."""
+    rows = max(1, max_q_len * group)
+    tiles = 1 if rows <= ROWS_ONE_TILE else ROWS_BLOCK // 16
+    blocks = -(-rows // (16 * tiles))
+    items = batch * kv_heads * blocks
+    most = min(MAX_SPLITS, max(1, -(-max_kv_len // MIN_SPLIT_KEYS)))
+    splits = max(1, min(most, -(-TARGET_WORKGROUPS // items)))
+    keys = max(64, -(-max_kv_len // splits))
+    keys = -(-keys // 64) * 64
+    return tiles, blocks, max(1, -(-max_kv_len // keys)), keys
+
+
+def workspace_bytes(batch: int, kv_heads: int, head_dim: int, shape: tuple[int, int, int, int]) -> int:
+    """Bytes of the split states of a call of ``shape`` (``launch_shape``)."""
+    tiles, blocks, splits, _ = shape
+    return 0 if splits == 1 else batch * kv_heads * blocks * splits * tiles * 16 * (4 * head_dim + 4)
+
+
+def _i32(t: torch.Tensor, name: str, count: int, device: torch.device) -> torch.Tensor:
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous int32 tensor")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.numel() != count:
+        raise ValueError(f"{name} has {t.numel()} entries, expected {count}")
+    return t
+
+
+def cache_geometry(paged_kv_cache, kv_layout: str):
+    """(K pages, V's byte offset, (page, token, head) byte strides, (pages, page
+    size, KV heads, head_dim)) of an NHD / HND cache, one tensor or a (K, V) pair."""
+    if kv_layout not in ("NHD", "HND"):
+        raise NotImplementedError(f"paged layout {kv_layout!r}: NHD and HND are supported")
+    if isinstance(paged_kv_cache, (tuple, list)):
+        base, v = paged_kv_cache
+        if base.shape != v.shape or base.stride() != v.stride() or base.dtype != v.dtype or base.device != v.device:
+            raise ValueError("K and V caches must have the same shape, strides, dtype and device")
+        if base.ndim != 4:
+            raise ValueError("tuple KV caches must be 4-dimensional")
+        v_offset = v.data_ptr() - base.data_ptr()
+    else:
+        base = paged_kv_cache
+        if base.ndim != 5 or base.shape[1] != 2:
+            raise ValueError(f"kv cache must be [pages, 2, ...] of {kv_layout} pages, got {tuple(base.shape)}")
+        v_offset = base.stride(1) * base.element_size()
+    es = base.element_size()
+    st, sh = base.stride(), base.shape
+    td, hd = (-3, -2) if kv_layout == "NHD" else (-2, -3)
+    if st[-1] != 1:
+        raise ValueError("kv cache head rows (D) must be contiguous")
+    return base, v_offset, (st[0] * es, st[td] * es, st[hd] * es), (sh[0], sh[td], sh[hd], sh[-1])
+
+
+def paged_attention(
+    q: torch.Tensor,
+    paged_kv_cache,
+    qo_indptr: torch.Tensor,
+    kv_indptr: torch.Tensor,
+    kv_indices: torch.Tensor,
+    kv_last_page_len: torch.Tensor,
+    *,
+    max_q_len: int | None = None,
+    max_kv_len: int | None = None,
+    kv_block_scales: torch.Tensor | None = None,
+    causal: bool = False,
+    tree_mask: torch.Tensor | None = None,
+    mask_col_start: torch.Tensor | None = None,
+    window_left: int = -1,
+    prefix_lens: torch.Tensor | None = None,
+    logits_soft_cap: float | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    sm_scale: float | None = None,
+    kv_layout: str = "NHD",
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+    return_lse: bool = False,
+    workspace: torch.Tensor | None = None,
+):
+    """Attention of a batch over its pages; returns ``out`` [nnz, Hq, D] (and
+    ``lse`` [nnz, Hq], natural logarithm).
+
+    ``q`` is [nnz, Hq, D] in fp16 or bf16, ``paged_kv_cache`` one tensor
+    [pages, 2, ...] or a (K, V) pair in ``kv_layout`` pages, of q's type or of
+    8-bit codes (float8_e4m3fn, int8) with ``kv_block_scales`` [pages, 2, Hkv]
+    in float32.  The four metadata arrays are int32 device tensors.
+
+    ``max_q_len`` and ``max_kv_len`` size the launch: a request with more queries
+    than ``max_q_len`` gets its first rows only, one with more keys than
+    ``max_kv_len`` is right but slower.  Left out, they are read back from the
+    metadata, which waits for the device (and cannot be captured).
+
+    Masks: none; ``causal`` with an optional ``window_left`` (keys more than that
+    far behind the query are hidden) and ``prefix_lens`` [batch] (keys below it
+    are visible to every query, also behind the window and ahead of the query); or
+    ``tree_mask`` with ``mask_col_start`` [batch] as the verify plans hold them: int64
+    [nnz] (bit j: key mask_col_start + j) or [nnz, words] (word j: keys
+    64 * (mask_col_start // 64 + j) ..).  A row that sees no key gets 0 and an
+    lse of -inf.  Rows past the last request's are left as they were.
+
+    ``workspace`` (uint8, ``workspace_bytes``) holds the split states; left out, it
+    comes from torch's allocator.  Calls that overlap must not share one."""
+    base, v_offset, (page_stride, token_stride, head_stride), (pages, page_size, hkv, d) = cache_geometry(
+        paged_kv_cache, kv_layout)
+    device = _lib.require_device(q, base, what="paged attention")
+    if q.ndim != 3 or q.stride(-1) != 1:
+        raise ValueError("q must be [nnz, Hq, D] with contiguous rows")
+    nnz, hq, qd = q.shape
+    if qd != d or hkv == 0 or hq % hkv != 0 or hq == 0:
+        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {hkv} KV heads of {d}")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    ss = (0, 0, 0)
+    if base.dtype in CACHE_CODES:
+        cache = CACHE_CODES[base.dtype]
+        s = kv_block_scales
+        if s is None:
+            raise ValueError("an 8-bit cache needs kv_block_scales")
+        if s.dtype != torch.float32 or tuple(s.shape) != (pages, 2, hkv) or s.device != device:
+            raise ValueError(f"kv_block_scales must be float32 [{pages}, 2, {hkv}] on {device}")
+        ss = s.stride()
+    elif base.dtype == q.dtype:
+        cache, s = _lib.CACHE_16BIT, None
+        if kv_block_scales is not None:
+            raise ValueError("kv_block_scales goes with an 8-bit cache")
+    else:
+        raise TypeError(f"a cache of {base.dtype} does not go with q of {q.dtype}")
+    batch = kv_last_page_len.numel()
+    if batch == 0:
+        raise ValueError("the batch must hold at least one request")
+    _i32(qo_indptr, "qo_indptr", batch + 1, device)
+    _i32(kv_indptr, "kv_indptr", batch + 1, device)
+    _i32(kv_last_page_len, "kv_last_page_len", batch, device)
+    _i32(kv_indices, "kv_indices", kv_indices.numel(), device)
+    mode, words = _lib.MASK_NONE, 1
+    if tree_mask is not None:
+        if causal or alibi_slopes is not None:
+            raise ValueError("a tree mask goes with neither causal nor a distance bias (its nodes stand in no order)")
+        if mask_col_start is None:
+            raise ValueError("tree_mask needs mask_col_start")
+        mode = _lib.MASK_TREE
+        words = 1 if tree_mask.ndim == 1 else tree_mask.shape[1]
+        if tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous() or tree_mask.ndim > 2 or \
+                tree_mask.shape[0] < nnz or words < 1 or tree_mask.device != device:
+            raise ValueError(f"tree_mask must be contiguous int64 [{nnz}] or [{nnz}, words] on {device}")
+        _i32(mask_col_start, "mask_col_start", batch, device)
+    elif causal:
+        mode = _lib.MASK_CAUSAL
+    if mode != _lib.MASK_CAUSAL and (window_left != -1 or prefix_lens is not None):
+        raise ValueError("window_left and prefix_lens go with causal=True")
+    if window_left < -1:
+        raise ValueError("window_left must be -1 (none) or not negative")
+    window_left = min(int(window_left), 1 << 30)
+    if prefix_lens is not None:
+        _i32(prefix_lens, "prefix_lens", batch, device)
+    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != hq
+                                     or not alibi_slopes.is_contiguous() or alibi_slopes.device != device):
+        raise ValueError(f"alibi_slopes must be contiguous float32 [{hq}] on {device}")
+    cap = 0.0 if logits_soft_cap is None else float(logits_soft_cap)
+    scale = 1.0 / math.sqrt(d) if sm_scale is None else float(sm_scale)
+    if not (0.0 <= cap < math.inf and -math.inf < scale < math.inf):
+        raise ValueError("logits_soft_cap must be finite and not negative, sm_scale finite")
+    if out is None:
+        out = torch.empty((nnz, hq, d), dtype=q.dtype, device=device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != device:
+        raise ValueError("out must have q's shape, dtype and device and contiguous rows")
+    if lse is None:
+        lse = torch.empty((nnz, hq), dtype=torch.float32, device=device) if return_lse else None
+    elif lse.dtype != torch.float32 or tuple(lse.shape) != (nnz, hq) or not lse.is_contiguous() or lse.device != device:
+        raise ValueError(f"lse must be contiguous float32 [{nnz}, {hq}]")
+    else:
+        return_lse = True
+    if nnz == 0:
+        return (out, lse) if return_lse else out
+    if max_q_len is None or max_kv_len is None:
+        qo, kvp, last = _host_lists(qo_indptr, kv_indptr, kv_last_page_len)
+        if max_q_len is None:
+            max_q_len = max(b - a for a, b in zip(qo, qo[1:]))
+        if max_kv_len is None:
+            max_kv_len = max((b - a - 1) * page_size + n if b > a else 0 for a, b, n in zip(kvp, kvp[1:], last))
+    if max_q_len < 0 or max_kv_len < 0:
+        raise ValueError("max_q_len and max_kv_len must not be negative")
+    max_q_len = min(int(max_q_len), nnz)
+    # (keys that a window leaves to a row block; the visible prefix comes on top)
+    reach = max_kv_len if window_left < 0 or prefix_lens is not None else min(max_kv_len, window_left + max_q_len)
+    tiles, blocks, splits, keys = shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach))
+    need = workspace_bytes(batch, hkv, d, shape)
+    if need:
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        elif workspace.device != device or not workspace.is_contiguous() or \
+                workspace.numel() * workspace.element_size() < need:
+            raise ValueError(f"the workspace must hold {need} contiguous bytes on {device}")
+    args = _ARGS.pack(
+        q.data_ptr(), base.data_ptr(), s.data_ptr() if s is not None else 0, qo_indptr.data_ptr(), kv_indptr.data_ptr(),
+        kv_indices.data_ptr(), kv_last_page_len.data_ptr(), tree_mask.data_ptr() if tree_mask is not None else 0,
+        mask_col_start.data_ptr() if mode == _lib.MASK_TREE else 0,
+        prefix_lens.data_ptr() if prefix_lens is not None else 0,
+        alibi_slopes.data_ptr() if alibi_slopes is not None else 0, out.data_ptr(),
+        lse.data_ptr() if lse is not None else 0, workspace.data_ptr() if need else 0,
+        need, q.stride(0), q.stride(1), out.stride(0), out.stride(1), page_stride, v_offset, token_stride, head_stride,
+        *ss, pages, kv_indices.numel(), nnz,
+        batch, hq, hkv, d, page_size, _lib.dtype_code(q.dtype), cache, mode, words, window_left, tiles, blocks, splits,
+        keys, scale, cap)
+    with _lib.on_device(device):
+        rc = _lib.load().atlas_paged_attn(args, _lib.stream_of(device))
+    _lib.check(rc, "atlas_paged_attn")
+    return (out, lse) if return_lse else out
+
+
+def default_alibi_slopes(num_qo_heads: int, device: torch.device) -> torch.Tensor:
+    """The usual slopes: 2^(-8 i / n), i = 1 .. n, for a power of two n of heads;
+    otherwise those of the next smaller power of two, then every other one of the next
+    larger."""
+    def geometric(n):
+        return [2.0 ** (-8.0 * i / n) for i in range(1, n + 1)]
+
+    n = 1 << (int(num_qo_heads).bit_length() - 1)
+    slopes = geometric(n) + geometric(2 * n)[0::2][: int(num_qo_heads) - n]
+    return torch.tensor(slopes, dtype=torch.float32, device=device)
+
+
+__all__ = ["paged_attention", "launch_shape", "workspace_bytes", "default_alibi_slopes"]

@@ -700,6 +700,109 @@ int atlas_candidate_select(const int64_t* parent_route_ids, const int64_t* stage
                            const int64_t* node_ids_dev, int64_t num_node_ids, int64_t* order_out,
                            int64_t* selected_out, int64_t* records_out, void* stream);
 
+/* ---- 8-bit caches and scored attention ------------------------------------
+ *
+ * An 8-bit cache holds K and V values as e4m3 (OCP fp8) or int8 with one fp32
+ * scale for each block, a block being one page's rows of one KV head and of K
+ * or V: the value is code * scale[page, kv, head].  Appends and commits write
+ * scales that are powers of two, so that a block whose scale grows is rounded
+ * once more at most by a whole number of binary places; attention takes any
+ * finite positive scale. */
+#define ATLAS_CACHE_16BIT 0
+#define ATLAS_CACHE_E4M3 1
+#define ATLAS_CACHE_INT8 2
+
+/* Arguments of atlas_paged_attn.  Pointers are device memory. */
+typedef struct {
+  const void* q; /* [nnz, Hq, D], rows contiguous */
+  const void* kv; /* page 0's first K row */
+  const float* kv_scales; /* [pages, 2, Hkv] (strides below), or NULL for a 16-bit cache */
+  const int32_t* qo_indptr; /* [batch + 1] */
+  const int32_t* kv_indptr; /* [batch + 1] */
+  const int32_t* kv_indices; /* page ids */
+  const int32_t* kv_last_page_len; /* [batch] */
+  const uint64_t* tree_mask; /* [nnz * mask_words], or NULL */
+  const int32_t* mask_col_start; /* [batch] with tree_mask */
+  const int32_t* prefix_lens; /* [batch], or NULL: keys below it are visible to every query */
+  const float* alibi_slopes; /* [Hq], or NULL */
+  void* out; /* [nnz, Hq, D] in q's dtype */
+  float* lse; /* [nnz, Hq] natural log, or NULL */
+  void* workspace; /* split states, NULL when num_splits is 1 */
+  int64_t workspace_bytes;
+  int64_t q_stride_token, q_stride_head; /* elements */
+  int64_t out_stride_token, out_stride_head; /* elements */
+  int64_t page_stride, v_offset, token_stride, head_stride; /* bytes */
+  int64_t scale_stride_page, scale_stride_kv, scale_stride_head; /* elements */
+  int64_t num_pages, num_indices, nnz;
+  int32_t batch, num_qo_heads, num_kv_heads, head_dim, page_size;
+  int32_t dtype; /* ATLAS_DTYPE_* of q and out (and of a 16-bit cache) */
+  int32_t cache; /* ATLAS_CACHE_* */
+  int32_t mask_mode; /* 0 none, 1 tree, 2 causal */
+  int32_t mask_words;
+  int32_t window_left; /* causal: keys below position - window_left are hidden; -1 none */
+  int32_t row_tiles; /* 1 or 4: query rows of a workgroup in tiles of 16 */
+  int32_t row_blocks; /* workgroups along a request's packed rows (query token * group + head of the group) */
+  int32_t num_splits; /* most key splits of a row block */
+  int32_t split_keys; /* least keys of a split, a multiple of 64 */
+  float sm_scale;
+  float soft_cap; /* 0: none; else scores become cap * tanh(score / cap) */
+} atlas_paged_attn_t;
+
+/* Attention over a paged cache from device-side metadata alone (no plan):
+ *   s = sm_scale * q . k;  s = soft_cap * tanh(s / soft_cap);
+ *   s -= alibi_slopes[head] * |position(q) - position(k)|
+ * softmax over the visible keys, times V.  Query i of a request with n queries
+ * and L keys has position L - n + i.  Causal: keys up to the query's position
+ * and not below it by more than window_left, and keys below prefix_lens.  Tree:
+ * as atlas_tree_verify_attn.  Rows that see no key get 0 and -inf.  Page ids
+ * outside [0, num_pages) are read as the nearest valid page and table entries
+ * past num_indices are not read.  A request's rows past row_blocks *
+ * row_tiles * 16 are not written.  Extends the paged decode / verify calls of
+ * flashinfer_full_verify.py:877-927 and sglang_page_attention.py:121-209. */
+int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream);
+/* Workspace bytes of a split row: head_dim fp32 values and an fp32 LSE. */
+#define ATLAS_PAGED_ATTN_ROW_BYTES(head_dim) (4 * (head_dim) + 4)
+
+/* Most items of one request in atlas_kv_commit_quantized. */
+#define ATLAS_QUANT_COMMIT_MAX_ITEMS 64
+
+/* Quantising append: the last append_indptr[b + 1] - append_indptr[b] positions
+ * of request b (its length comes from kv_indptr and kv_last_page_len) take the
+ * rows k_src / v_src [append_indptr[b] ..] (dtype f16 or bf16, rows of
+ * num_kv_heads * head_dim contiguous), every layer.  A block's scale is the
+ * least power of two under which its new rows fit (e4m3: 448, int8: 127), and not
+ * less than the block's scale if it holds older rows; those are then rounded to the
+ * new scale.  Rows are rounded to nearest, ties to even; infinities become the
+ * largest value and do not count for the scale, NaN stays NaN in e4m3 and
+ * becomes 0 in int8.  Bytes behind a request's last row stay as they are.
+ * max_append: most rows of one request (rows past it are not written).
+ * head_stride and the scales' strides as in atlas_paged_attn_t.  Replaces
+ * write_suffix_kv / set_kv_buffer for such caches. */
+int atlas_kv_append_quantized(const void* const* layers, const void* const* scales, int num_layers, int cache,
+                              int64_t page_size, int64_t page_stride, int64_t v_offset, int64_t token_stride,
+                              int64_t head_stride, int64_t scale_stride_page, int64_t scale_stride_kv,
+                              int64_t scale_stride_head, const void* const* k_src, const void* const* v_src,
+                              int64_t src_token_stride, int dtype, int num_kv_heads, int head_dim,
+                              const int32_t* append_indptr_dev, const int32_t* kv_indptr_dev,
+                              const int32_t* kv_indices_dev, const int32_t* kv_last_page_len_dev, int batch,
+                              int64_t max_append, int64_t nnz, int64_t num_pages, int64_t num_indices, void* stream);
+
+/* Route commit in an 8-bit cache: row src_pos[i] of request b moves to dst_pos[i]
+ * for items item_indptr[b] <= i < item_indptr[b + 1] (all sources are read before
+ * any row of the request is written), every layer.  A destination block's scale
+ * becomes the largest of its own and its moved rows' source blocks; when it
+ * grows, the block's other rows are rounded to it.  Items with a position or
+ * page outside the request's table or the pool are skipped.  Requests must not
+ * share destination pages.  Replaces target_kv_commit (target_runtime.py:910-912)
+ * for such caches. */
+int atlas_kv_commit_quantized(const void* const* layers, const void* const* scales, int num_layers, int cache,
+                              int64_t page_size, int64_t page_stride, int64_t v_offset, int64_t token_stride,
+                              int64_t head_stride, int64_t scale_stride_page, int64_t scale_stride_kv,
+                              int64_t scale_stride_head, int num_kv_heads, int head_dim, const int64_t* src_pos_dev,
+                              const int64_t* dst_pos_dev, const int32_t* item_indptr_dev, const int32_t* kv_indptr_dev,
+                              const int32_t* kv_indices_dev, int batch, int max_items, int64_t num_items,
+                              int64_t num_pages, int64_t num_indices, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
