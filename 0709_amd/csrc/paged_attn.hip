@@ -1,6 +1,6 @@
 // Paged attention from device-side metadata: argument checks, and the kernels
-// over 16-bit caches (paged_attn.hpp).
-#include "paged_attn.hpp"
+// over 16-bit caches.
+#include "paged_launch.hpp"
 
 namespace atlas {
 
@@ -38,7 +38,9 @@ extern "C" int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream) {
   ATLAS_REQUIRE(p.mask_mode == 2 || (p.window_left < 0 && p.prefix_lens == nullptr),
                 "windows and prefixes go with the causal mask");
   ATLAS_REQUIRE(p.mask_mode != 1 || p.alibi_slopes == nullptr, "a distance bias does not go with a tree mask");
-  ATLAS_REQUIRE(p.row_tiles == 1 || p.row_tiles == 4, "row_tiles must be 1 or 4");
+  ATLAS_REQUIRE(p.block_rows > 0 && p.block_rows % 16 == 0 && p.block_rows <= (p.single_token ? 16 : 128),
+                "block_rows must be a multiple of 16, up to 128 (16 for single tokens), got %d", p.block_rows);
+  ATLAS_REQUIRE(!p.single_token || p.mask_mode != 1, "single_token does not go with a tree mask");
   ATLAS_REQUIRE(p.row_blocks > 0 && p.num_splits > 0 && p.split_keys > 0 && p.split_keys % 64 == 0,
                 "row_blocks, num_splits and split_keys (a multiple of 64) must be positive");
   ATLAS_REQUIRE(p.soft_cap >= 0.f, "soft_cap must not be negative");
@@ -59,7 +61,7 @@ extern "C" int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream) {
     return ATLAS_EUNSUPPORTED;
   }
   const int64_t blocks = int64_t(p.batch) * p.num_kv_heads * p.row_blocks;
-  const int64_t rows = blocks * p.num_splits * p.row_tiles * 16;
+  const int64_t rows = blocks * p.num_splits * p.block_rows;
   if (blocks * p.num_splits >= (int64_t(1) << 23)) {
     set_error("%lld workgroups are too many", static_cast<long long>(blocks * p.num_splits));
     return ATLAS_EUNSUPPORTED;

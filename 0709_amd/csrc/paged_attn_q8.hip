@@ -1,5 +1,5 @@
-// Paged attention over 8-bit caches (kernel in paged_attn.hpp).
-#include "paged_attn.hpp"
+// Paged attention over 8-bit caches.
+#include "paged_launch.hpp"
 
 namespace atlas {
 

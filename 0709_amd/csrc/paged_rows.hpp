@@ -1,0 +1,488 @@
+// Paged attention for several query tokens per request: prompts' chunks, draft
+// trees, short batches.
+//
+// A workgroup of four waves takes up to 64 * RT packed rows of one KV head and one
+// split of the request's keys.  Tiles of 64 keys go from HBM through registers into
+// LDS as 16-bit rows (8-bit codes are converted on the way, once for all rows), one
+// tile ahead of the products, in two stages: the tile's loads are in flight while the
+// one before it is computed.  Row tiles of 16 go round the waves; K's operand is a
+// 16-byte LDS read, V's two transposing reads.  A row's 16-byte granules are swapped
+// by the key so that neither the writes nor either kind of read meets in a bank.
+#pragma once
+
+#include "paged_attn.hpp"
+
+namespace atlas {
+namespace {
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ w2 read_tr16(const char* p) {
+  return __builtin_bit_cast(w2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (__attribute__((address_space(3))) s4*)(p)));
+}
+
+// LDS writes of every wave are visible behind it; loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// Bits of the four keys key0 .. key0 + 3 below `end`.
+__device__ __forceinline__ uint32_t below4(int key0, int end) {
+  return (1u << min(max(end - key0, 0), 4)) - 1u;
+}
+
+template <int KIND, int D, int RT, bool PAGE16>
+__global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs a) {
+  typedef Cache<KIND> C;
+  typedef typename C::frag frag;
+  constexpr bool Q8 = C::kQuant;
+  constexpr int TK = kChunk;               // keys of a tile
+  constexpr int KS = D / 32;               // steps of the score product
+  constexpr int DT = D / 16;               // 16-dim tiles of O
+  constexpr int RB = D * 2;                // bytes of an LDS row
+  constexpr int GR = RB / 16;              // its granules
+  constexpr int HALF = TK * RB;            // K's or V's half of a stage
+  constexpr int GG = D * C::kBytes / 16;   // 16-byte pieces of a row in the cache
+  constexpr int NL = TK * GG / kPaThreads; // pieces a thread carries, of K and of V
+  constexpr int KSW = GR - 1;              // granule swaps: K by key, V by key pairs
+  constexpr int VSW = GR / 2 - 1;
+  const atlas_paged_attn_t& p = a.p;
+
+  __shared__ __attribute__((aligned(16))) char lds[2][2 * HALF];
+  constexpr int NSC = PAGE16 ? 4 : TK;     // scales of a tile: by 16 keys, or by key
+  __shared__ __attribute__((aligned(16))) float scale_lds[2][2][NSC];
+  __shared__ int strange_lds[2];
+
+  // Row blocks of one (request, head, split) stream the same keys: they run next to
+  // each other on one XCD (workgroups go round the 8 XCDs).
+  int unit, rb;
+  if (p.row_blocks == 1) {
+    unit = blockIdx.x;
+    rb = 0;
+  } else {
+    const int j = blockIdx.x >> 3;
+    rb = j % p.row_blocks;
+    unit = (j / p.row_blocks) * 8 + (blockIdx.x & 7);
+  }
+  const int h = unit % p.num_kv_heads;
+  const int split = (unit / p.num_kv_heads) % p.num_splits;
+  const int b = unit / p.num_kv_heads / p.num_splits;
+  if (b >= p.batch) return;
+  const Request r = read_request(p, b);
+  const int row_start = rb * p.block_rows;
+  const int rows = min(p.block_rows, r.q_len * a.group - row_start);
+  if (rows <= 0) return;
+  const Block k = plan_block(a, r, b, row_start, rows);
+  if (split >= k.splits) return;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, r16 = lane & 15;
+  const bool bf16 = p.dtype == ATLAS_DTYPE_BF16;
+  const int shift = r.kv_len - r.q_len;  // position of query token 0
+  const int col0 = p.mask_mode == 1 ? p.mask_col_start[b] : 0;
+  // this wave's row tiles: wave, wave + 4
+  const int tiles = (rows + 15) / 16;
+  const int nrt = tiles > wave ? (tiles - wave + 3) / 4 : 0;
+
+  // ---- queries ----
+  frag qf[RT][KS];
+  float qscale[RT], m_run[RT], l_run[RT], slope[RT];
+  f32x4 o[RT][DT];
+  int node_of[RT], head_of[RT];
+  uint64_t word[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = (wave + 4 * rt) * 16 + r16;
+    const bool ok = row < rows;
+    const int prow = row_start + (ok ? row : 0);
+    node_of[rt] = prow / a.group;
+    head_of[rt] = h * a.group + (prow - node_of[rt] * a.group);
+    const char* qrow = static_cast<const char*>(p.q) +
+                       (int64_t(r.q0 + node_of[rt]) * p.q_stride_token + int64_t(head_of[rt]) * p.q_stride_head) * 2;
+    qscale[rt] = a.scale_log2;
+    w4 v[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      v[ks] = *reinterpret_cast<const w4*>(qrow + (ks * 32 + g * 8) * 2);
+      if (!ok) v[ks] = w4{0, 0, 0, 0};
+    }
+    if constexpr (Q8) {
+      float f[KS][8];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) q_floats(v[ks], bf16, f[ks]);
+      qscale[rt] *= q_to_f16<KS>(f, qf[rt]);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = v[ks];
+    }
+    m_run[rt] = -INFINITY;
+    l_run[rt] = 0.f;
+    slope[rt] = p.alibi_slopes ? p.alibi_slopes[head_of[rt]] * kPaLog2e : 0.f;
+    word[rt] = (p.mask_mode == 1 && p.mask_words == 1 && ok) ? p.tree_mask[r.q0 + node_of[rt]] : 0ull;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // ---- keys ----
+  const char* kbase = static_cast<const char*>(p.kv) + int64_t(h) * p.head_stride;
+  const char* vbase = kbase + p.v_offset;
+  const int ts = int(p.token_stride);
+  const int page_size = p.page_size;
+  auto slot_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / page_size; };
+  PageWindow<Q8> pages;
+  pages.ids = p.kv_indices + r.pt;
+  pages.scales = Q8 ? p.kv_scales + int64_t(h) * p.scale_stride_head : nullptr;
+  pages.scale_page = p.scale_stride_page;
+  pages.scale_kv = p.scale_stride_kv;
+  pages.last_id = p.num_pages - 1;
+  pages.lane = lane;
+  pages.last_slot = k.hi > 0 ? slot_of(max(k.hi, k.prefix) - 1) : 0;
+
+  auto key_of = [&](int c) { return (c < k.ca ? c : c - k.ca + k.cb) * TK; };
+  auto bounds = [&](int c, int& lo, int& hi) {
+    lo = c < k.ca ? 0 : k.lo;
+    hi = (c < k.ca ? k.prefix : k.hi) - 1;
+  };
+  // Piece j of a thread: row (j * 256 + tid) / GG of the tile, piece tid % GG of it.
+  const int piece = tid % GG, prow0 = tid / GG;
+  constexpr int RSTEP = kPaThreads / GG;  // rows between a thread's pieces
+  w4 kraw[NL], vraw[NL];
+  float ksc[PAGE16 ? 4 : 1], vsc[PAGE16 ? 4 : 1];  // scales of its 16-key tiles, or of key tid / 4
+  // Keys outside [lo, hi) of the tile's part repeat its nearest key.
+  auto load = [&](int c) {
+    const int kb = key_of(c);
+    int lo, hi;
+    bounds(c, lo, hi);
+    if constexpr (PAGE16) pages.reach(slot_of(min(max(kb + TK - 16, lo & ~15), hi & ~15)));
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
+      int64_t at;
+      if constexpr (PAGE16) {
+        // (a wave's rows of one piece lie in one 16-key tile)
+        const int t0 = kb + ((j * RSTEP + wave * (64 / GG)) & ~15);
+        const int slot = slot_of(min(max(t0, lo & ~15), hi & ~15));
+        at = int64_t(pages.id(slot)) * p.page_stride + uint32_t((key - slot * page_size) * ts + piece * 16);
+      } else {
+        const int slot = slot_of(key);
+        const int64_t id = pages.ids[slot];
+        at = (id < 0 ? 0 : (id > pages.last_id ? pages.last_id : id)) * p.page_stride +
+             int64_t(key - slot * page_size) * ts + piece * 16;
+      }
+      kraw[j] = *reinterpret_cast<const w4*>(kbase + at);
+      vraw[j] = *reinterpret_cast<const w4*>(vbase + at);
+    }
+    if constexpr (Q8 && PAGE16) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        const int slot = slot_of(min(max(kb + kt * 16, lo & ~15), hi & ~15));
+        ksc[kt] = pages.k_scale(slot);
+        vsc[kt] = pages.v_scale(slot);
+      }
+    } else if constexpr (Q8) {
+      const int slot = slot_of(min(max(kb + (tid >> 2), lo), hi));
+      const int64_t id = pages.ids[slot];
+      const float* s = pages.scales + (id < 0 ? 0 : (id > pages.last_id ? pages.last_id : id)) * p.scale_stride_page;
+      ksc[0] = s[0];
+      vsc[0] = s[p.scale_stride_kv];
+    }
+  };
+  // Does some key of tile c hide from some row?
+  auto masked_tile = [&](int kb) {
+    if (p.mask_mode == 2)
+      return !(kb + TK <= k.prefix || (kb + TK <= shift + k.n0 + 1 &&
+                                       (p.window_left < 0 || kb >= shift + k.n1 - p.window_left)));
+    return kb + TK > (p.mask_mode == 1 ? min(r.kv_len, col0) : r.kv_len);
+  };
+  auto store = [&](int st, int c) {
+    char* kd = lds[st];
+    char* vd = lds[st] + HALF;
+    // Infinities and NaN in V rows that a row does not see must not reach it
+    // (0 * inf): tiles with hidden keys that hold some are marked.
+    bool odd = false;
+    const bool look = KIND != kCacheInt8 && masked_tile(key_of(c));
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int row = j * RSTEP + prow0;
+      if constexpr (!Q8) {
+        *reinterpret_cast<w4*>(kd + row * RB + ((piece ^ (row & KSW)) << 4)) = kraw[j];
+        *reinterpret_cast<w4*>(vd + row * RB + ((piece ^ ((row & VSW) << 1)) << 4)) = vraw[j];
+        if (look) {
+          constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) odd |= (vraw[j][w] & kExp) == kExp || ((vraw[j][w] >> 16) & kExp) == kExp;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int gr = 2 * piece + e;
+          *reinterpret_cast<frag*>(kd + row * RB + ((gr ^ (row & KSW)) << 4)) = C::keys8(kraw[j][2 * e], kraw[j][2 * e + 1]);
+          *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = C::keys8(vraw[j][2 * e], vraw[j][2 * e + 1]);
+        }
+        if (KIND == kCacheE4M3 && look) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd |= ((vraw[j][w] >> (8 * e)) & 0x7fu) == 0x7fu;
+        }
+      }
+    }
+    if constexpr (Q8 && PAGE16) {
+      if (tid == 0) {
+        *reinterpret_cast<f32x4*>(scale_lds[st][0]) = f32x4{ksc[0], ksc[1], ksc[2], ksc[3]};
+        *reinterpret_cast<f32x4*>(scale_lds[st][1]) = f32x4{vsc[0], vsc[1], vsc[2], vsc[3]};
+      }
+    } else if constexpr (Q8) {
+      if ((tid & 3) == 0) {
+        scale_lds[st][0][tid >> 2] = ksc[0];
+        scale_lds[st][1][tid >> 2] = vsc[0];
+      }
+    }
+    if (look && odd) strange_lds[st] = c + 1;
+  };
+
+  // Largest V scale so far: O holds sums of p * v * (scale / vref).
+  float vref = 1.17549435e-38f, vinv = 8.5070592e37f;
+
+  // Lane parts of the LDS addresses: K row r16 of a 16-key tile, V rows 4g + r16 / 4.
+  const int e4 = r16 >> 2, q4 = r16 & 3;
+  const int vkey = 4 * g + e4;
+
+  // One tile for this wave's first NR row tiles.
+  auto compute = [&](auto nr_tag, int st, int c) {
+    constexpr int NR = decltype(nr_tag)::value;
+    const int kb = key_of(c);
+    const char* kd = lds[st];
+    const char* vd = lds[st] + HALF;
+    f32x4 acc[NR][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+      for (int rt = 0; rt < NR; ++rt) acc[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const frag kf = *reinterpret_cast<const frag*>(kd + (kt * 16 + r16) * RB + (((ks * 4 + g) ^ (r16 & KSW)) << 4));
+#pragma unroll
+        for (int rt = 0; rt < NR; ++rt) acc[rt][kt] = C::mfma(kf, qf[rt][ks], acc[rt][kt]);
+      }
+    }
+    f32x4 ksk[PAGE16 ? 1 : 4], vsk[PAGE16 ? 1 : 4];  // scales of the 16-key tiles, or of the lane's keys
+    if constexpr (Q8) {
+#pragma unroll
+      for (int kt = 0; kt < (PAGE16 ? 1 : 4); ++kt) {
+        ksk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][0][PAGE16 ? 0 : kt * 16 + 4 * g]);
+        vsk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][1][PAGE16 ? 0 : kt * 16 + 4 * g]);
+      }
+      float top = vsk[0][0];
+#pragma unroll
+      for (int i = 1; i < (PAGE16 ? 4 : 16); ++i) top = fmaxf(top, vsk[i >> 2][i & 3]);
+      if constexpr (!PAGE16) top = groups_max(top);
+      if (__builtin_amdgcn_ballot_w64(top > vref) != 0) {
+        const float down = vref / top;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int t = 0; t < DT; ++t) o[rt][t] *= down;
+        vref = top;
+        vinv = 1.0f / top;
+      }
+    }
+    const bool masked = masked_tile(kb);
+    frag pf[NR][2];
+#pragma unroll
+    for (int rt = 0; rt < NR; ++rt) {
+      float sc[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float f = qscale[rt];
+        if constexpr (Q8) f *= PAGE16 ? ksk[0][i >> 2] : ksk[PAGE16 ? 0 : i >> 2][i & 3];
+        sc[i] = acc[rt][i >> 2][i & 3] * f;
+      }
+      if (p.soft_cap > 0.f) {
+        // cap * tanh(y / cap) = cap * (1 - 2 / (1 + e^(2 y / cap))), to powers of two
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(sc[i] * a.cap_in);
+          sc[i] = __builtin_fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(1.f + e), a.cap_out);
+        }
+      }
+      const int qpos = shift + node_of[rt];
+      const int key0 = kb + 4 * g;
+      if (p.alibi_slopes != nullptr) {
+        const float away = float(qpos - key0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          sc[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), sc[i]);
+      }
+      if (masked) {
+        uint64_t w = word[rt];
+        int w0 = col0;
+        if (p.mask_mode == 1 && p.mask_words > 1) {
+          // one word for each 64 keys, and a tile is one of them
+          const int idx = (kb >> 6) - (col0 >> 6);
+          w = idx < 0 ? ~0ull
+                      : (idx < p.mask_words && (wave + 4 * rt) * 16 + r16 < rows
+                             ? p.tree_mask[int64_t(r.q0 + node_of[rt]) * p.mask_words + idx] : 0ull);
+          w0 = kb;
+        }
+        const int wlo = p.window_left >= 0 ? qpos - p.window_left : 0;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          const int at = key0 + kt * 16;
+          uint32_t vis = below4(at, r.kv_len);
+          if (p.mask_mode == 2) {
+            vis &= (below4(at, qpos + 1) & ~below4(at, wlo)) | below4(at, k.prefix);
+          } else if (p.mask_mode == 1) {
+            const int off = at - w0;  // the lane's keys in the word; those before it are the prefix
+            const int pre = min(max(-off, 0), 4);
+            const uint32_t up = off >= 0 && off < 64 ? uint32_t(w >> (off & 63)) : 0u;
+            const uint32_t down = uint32_t(w << pre) | ((1u << pre) - 1u);
+            vis &= off >= 0 ? up : down;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[kt * 4 + i] = (vis >> i) & 1u ? sc[kt * 4 + i] : -INFINITY;
+        }
+      }
+      float mx = sc[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = pa_max(mx, sc[i]);
+      if (__builtin_amdgcn_ballot_w64(mx > m_run[rt] + kPaLazyLog2) != 0) {
+        const float top = groups_max(mx);
+        const bool grow = top > m_run[rt] + kPaLazyLog2;  // (a row's results do not depend on its neighbours)
+        const float m_new = grow ? top : m_run[rt];
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[rt] - m_new) : 1.f;
+        l_run[rt] *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[rt][t] *= alpha;
+        m_run[rt] = m_new;
+      }
+      const float m = m_run[rt] == -INFINITY ? 0.f : m_run[rt];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(sc[kt * 4 + i] - m);
+          l_run[rt] += e[i];
+          if constexpr (Q8) e[i] *= (PAGE16 ? vsk[0][kt] : vsk[PAGE16 ? 0 : kt][i]) * vinv;
+        }
+        pf[rt][kt >> 1][(kt & 1) * 2] = C::pack(e[0], e[1]);
+        pf[rt][kt >> 1][(kt & 1) * 2 + 1] = C::pack(e[2], e[3]);
+      }
+    }
+    // V^T's operand of dim tile t and the keys 32 hh .. + 31 of the tile
+    auto v_frag = [&](int t, int hh) {
+      const char* at = vd + (32 * hh + vkey) * RB + (((2 * t + (q4 >> 1)) ^ ((vkey & VSW) << 1)) << 4) + ((q4 & 1) << 3);
+      const w2 x = read_tr16(at), y = read_tr16(at + 16 * RB);
+      return frag{x[0], x[1], y[0], y[1]};
+    };
+    if (!(masked && KIND != kCacheInt8 && strange_lds[st] == c + 1)) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const frag vf = v_frag(t, hh);
+#pragma unroll
+          for (int rt = 0; rt < NR; ++rt) o[rt][t] = C::mfma(vf, pf[rt][hh], o[rt][t]);
+        }
+    } else {
+      // finite values as they are; where a row that sees the key has an infinity or
+      // NaN, its sum becomes one
+      constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u, kOne = C::kBf16 ? 0x3f80u : 0x3c00u;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const frag vf = v_frag(t, hh);
+          frag fine, up, dn;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            fine[j] = up[j] = dn[j] = 0;
+#pragma unroll
+            for (int hw = 0; hw < 2; ++hw) {
+              const uint32_t v = (vf[j] >> (16 * hw)) & 0xffffu;
+              const bool bad = (v & kExp) == kExp, nan = (v & 0x7fffu) > kExp;
+              fine[j] |= (bad ? 0u : v) << (16 * hw);
+              up[j] |= (bad && (nan || v == kExp) ? kOne : 0u) << (16 * hw);
+              dn[j] |= (bad && (nan || v != kExp) ? kOne : 0u) << (16 * hw);
+            }
+          }
+#pragma unroll
+          for (int rt = 0; rt < NR; ++rt) {
+            const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+            o[rt][t] = C::mfma(fine, pf[rt][hh], o[rt][t]);
+            const f32x4 plus = C::mfma(up, pf[rt][hh], zero), minus = C::mfma(dn, pf[rt][hh], zero);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (plus[i] > 0.f) o[rt][t][i] += INFINITY;
+              if (minus[i] > 0.f) o[rt][t][i] -= INFINITY;
+            }
+          }
+        }
+    }
+  };
+
+  const int c0 = split * k.per, c1 = min(k.chunks, c0 + k.per);
+  if (c0 < c1) {
+    if (tid < 2) strange_lds[tid] = 0;
+    if constexpr (PAGE16) {
+      int lo, hi;
+      bounds(c0, lo, hi);
+      pages.begin(slot_of(min(max(key_of(c0), lo), hi)));
+    }
+    load(c0);
+    lds_barrier();  // (the marks are cleared)
+    store(0, c0);
+    if (c0 + 1 < c1) load(c0 + 1);
+    lds_barrier();
+    for (int c = c0; c < c1; ++c) {
+      const int st = (c - c0) & 1;
+      // the next tile's registers go to the other stage, which every wave left
+      // before the last barrier; then the one behind it is asked for
+      if (c + 1 < c1) store(st ^ 1, c + 1);
+      if (c + 2 < c1) load(c + 2);
+      if (nrt == 1) compute(std::integral_constant<int, 1>{}, st, c);
+      if constexpr (RT == 2) {
+        if (nrt == 2) compute(std::integral_constant<int, 2>{}, st, c);
+      }
+      lds_barrier();
+    }
+  }
+
+  // ---- results ----
+  const int64_t item = (int64_t(b) * p.num_kv_heads + h) * p.row_blocks + rb;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int lr = (wave + 4 * rt) * 16 + r16;
+    const float sum = groups_sum(l_run[rt]);
+    if (lr >= rows) continue;
+    const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (Q8 ? vref : 1.f);
+    const float lse2 = sum == 0.f ? -INFINITY : m_run[rt] + __builtin_log2f(sum);
+    if (k.splits > 1) {
+      float* ws = static_cast<float*>(p.workspace);
+      const int64_t prow = (item * p.num_splits + split) * p.block_rows + lr;
+      const int64_t nrows = int64_t(p.batch) * p.num_kv_heads * p.row_blocks * p.num_splits * p.block_rows;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(ws + prow * D + t * 16 + 4 * g) = o[rt][t] * inv;
+      if (g == 0) ws[nrows * D + prow] = lse2;
+    } else {
+      char* out = static_cast<char*>(p.out) + (int64_t(r.q0 + node_of[rt]) * p.out_stride_token +
+                                               int64_t(head_of[rt]) * p.out_stride_head) * 2;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const f32x4 x = o[rt][t] * inv;
+        *reinterpret_cast<w2*>(out + (t * 16 + 4 * g) * 2) =
+            bf16 ? w2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])} : w2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])};
+      }
+      if (p.lse != nullptr && g == 0)
+        p.lse[int64_t(r.q0 + node_of[rt]) * p.num_qo_heads + head_of[rt]] = lse2 * kPaLn2;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace atlas

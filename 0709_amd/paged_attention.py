@@ -32,10 +32,9 @@ import torch
 from . import _lib
 from .tree_attention import _host_lists
 
-# Packed query rows (query token * group + head of the group) of one workgroup, in
-# row tiles of 16.
-ROWS_ONE_TILE = 16
-ROWS_BLOCK = 64
+# Most packed query rows (query token * group + head of the group) of a workgroup.
+DECODE_ROWS = 16
+BLOCK_ROWS = 128
 # Workgroups to aim for when the keys are split, and the least keys of a split.
 TARGET_WORKGROUPS = 1024
 MIN_SPLIT_KEYS = 256
@@ -43,32 +42,34 @@ MAX_SPLITS = 256
 
 CACHE_CODES = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
 
-# atlas_paged_attn_t: 14 pointers, 15 int64, 14 int32, 2 floats
-_ARGS = struct.Struct("=14P15q14i2f".replace("P", "Q"))
+# atlas_paged_attn_t: 14 pointers, 15 int64, 15 int32, 2 floats
+_ARGS = struct.Struct("=14Q15q15i2f4x")
 
 
-def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int) -> tuple[int, int, int, int]:
-    """(row tiles, row blocks, splits, keys per split) of a call.
+def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int,
+                 tree: bool = False) -> tuple[bool, int, int, int, int]:
+    """(single token?, rows of a block, row blocks, splits, keys per split) of a call.
 
-    Up to 16 packed rows take the one-tile kernel, more the four-tile one.  Keys
-    are split until about TARGET_WORKGROUPS workgroups are there, in splits of at
-    least MIN_SPLIT_KEYS; a request shorter than ``max_kv_len`` takes fewer
-    splits of the same size."""
+    One query token per request takes the decode kernel with blocks of 16 packed
+    rows.  More take equal blocks of up to BLOCK_ROWS.  Keys are split until about
+    TARGET_WORKGROUPS workgroups are there, in splits of at least MIN_SPLIT_KEYS;
+    a request shorter than ``max_kv_len`` takes fewer splits of the same size."""
+    single = max_q_len <= 1 and not tree
     rows = max(1, max_q_len * group)
-    tiles = 1 if rows <= ROWS_ONE_TILE else ROWS_BLOCK // 16
-    blocks = -(-rows // (16 * tiles))
+    blocks = -(-rows // (DECODE_ROWS if single else BLOCK_ROWS))
+    block_rows = DECODE_ROWS if single else 16 * -(-rows // (16 * blocks))
     items = batch * kv_heads * blocks
     most = min(MAX_SPLITS, max(1, -(-max_kv_len // MIN_SPLIT_KEYS)))
     splits = max(1, min(most, -(-TARGET_WORKGROUPS // items)))
     keys = max(64, -(-max_kv_len // splits))
     keys = -(-keys // 64) * 64
-    return tiles, blocks, max(1, -(-max_kv_len // keys)), keys
+    return single, block_rows, blocks, max(1, -(-max_kv_len // keys)), keys
 
 
-def workspace_bytes(batch: int, kv_heads: int, head_dim: int, shape: tuple[int, int, int, int]) -> int:
+def workspace_bytes(batch: int, kv_heads: int, head_dim: int, shape: tuple[bool, int, int, int, int]) -> int:
     """Bytes of the split states of a call of ``shape`` (``launch_shape``)."""
-    tiles, blocks, splits, _ = shape
-    return 0 if splits == 1 else batch * kv_heads * blocks * splits * tiles * 16 * (4 * head_dim + 4)
+    _, block_rows, blocks, splits, _ = shape
+    return 0 if splits == 1 else batch * kv_heads * blocks * splits * block_rows * (4 * head_dim + 4)
 
 
 def _i32(t: torch.Tensor, name: str, count: int, device: torch.device) -> torch.Tensor:
@@ -237,7 +238,7 @@ def paged_attention(
     max_q_len = min(int(max_q_len), nnz)
     # (keys that a window leaves to a row block; the visible prefix comes on top)
     reach = max_kv_len if window_left < 0 or prefix_lens is not None else min(max_kv_len, window_left + max_q_len)
-    tiles, blocks, splits, keys = shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach))
+    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach), mode == _lib.MASK_TREE)
     need = workspace_bytes(batch, hkv, d, shape)
     if need:
         if workspace is None:
@@ -254,8 +255,8 @@ def paged_attention(
         lse.data_ptr() if lse is not None else 0, workspace.data_ptr() if need else 0,
         need, q.stride(0), q.stride(1), out.stride(0), out.stride(1), page_stride, v_offset, token_stride, head_stride,
         *ss, pages, kv_indices.numel(), nnz,
-        batch, hq, hkv, d, page_size, _lib.dtype_code(q.dtype), cache, mode, words, window_left, tiles, blocks, splits,
-        keys, scale, cap)
+        batch, hq, hkv, d, page_size, _lib.dtype_code(q.dtype), cache, mode, words, window_left,
+        *shape, scale, cap)
     with _lib.on_device(device):
         rc = _lib.load().atlas_paged_attn(args, _lib.stream_of(device))
     _lib.check(rc, "atlas_paged_attn")

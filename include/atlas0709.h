@@ -740,8 +740,9 @@ typedef struct {
   int32_t mask_mode; /* 0 none, 1 tree, 2 causal */
   int32_t mask_words;
   int32_t window_left; /* causal: keys below position - window_left are hidden; -1 none */
-  int32_t row_tiles; /* 1 or 4: query rows of a workgroup in tiles of 16 */
-  int32_t row_blocks; /* workgroups along a request's packed rows (query token * group + head of the group) */
+  int32_t single_token; /* 1: no request has more than one query token (later ones are not written) */
+  int32_t block_rows; /* packed rows (query token * group + head of the group) of a workgroup: a multiple of 16 up to 128, 16 with single_token */
+  int32_t row_blocks; /* workgroups along a request's packed rows */
   int32_t num_splits; /* most key splits of a row block */
   int32_t split_keys; /* least keys of a split, a multiple of 64 */
   float sm_scale;
@@ -757,7 +758,7 @@ typedef struct {
  * as atlas_tree_verify_attn.  Rows that see no key get 0 and -inf.  Page ids
  * outside [0, num_pages) are read as the nearest valid page and table entries
  * past num_indices are not read.  A request's rows past row_blocks *
- * row_tiles * 16 are not written.  Extends the paged decode / verify calls of
+ * block_rows are not written.  Extends the paged decode / verify calls of
  * flashinfer_full_verify.py:877-927 and sglang_page_attention.py:121-209. */
 int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream);
 /* Workspace bytes of a split row: head_dim fp32 values and an fp32 LSE. */
