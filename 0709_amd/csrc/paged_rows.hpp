@@ -54,7 +54,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   __shared__ __attribute__((aligned(16))) char lds[2][2 * HALF];
   constexpr int NSC = PAGE16 ? 4 : TK;     // scales of a tile: by 16 keys, or by key
   __shared__ __attribute__((aligned(16))) float scale_lds[2][2][NSC];
-  __shared__ int strange_lds[2];
+  __shared__ int strange_lds[2];             // tile (+ 1) of the stage that holds such values
+  __shared__ uint8_t up_lds[2][TK * D / 8];  // bits of V values that are +inf or NaN, by key and dim
+  __shared__ uint8_t dn_lds[2][TK * D / 8];  // -inf or NaN
 
   // Row blocks of one (request, head, split) stream the same keys: they run next to
   // each other on one XCD (workgroups go round the 8 XCDs).
@@ -84,25 +86,23 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const bool bf16 = p.dtype == ATLAS_DTYPE_BF16;
   const int shift = r.kv_len - r.q_len;  // position of query token 0
   const int col0 = p.mask_mode == 1 ? p.mask_col_start[b] : 0;
-  // this wave's row tiles: wave, wave + 4
-  const int tiles = (rows + 15) / 16;
-  const int nrt = tiles > wave ? (tiles - wave + 3) / 4 : 0;
+  // this wave's row tiles are wave, wave + 4 (one without rows computes with queries of zeros)
+  const bool computes = wave * 16 < rows;
 
   // ---- queries ----
   frag qf[RT][KS];
   float qscale[RT], m_run[RT], l_run[RT], slope[RT];
   f32x4 o[RT][DT];
-  int node_of[RT], head_of[RT];
-  uint64_t word[RT];
+  int node_of[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row = (wave + 4 * rt) * 16 + r16;
     const bool ok = row < rows;
     const int prow = row_start + (ok ? row : 0);
     node_of[rt] = prow / a.group;
-    head_of[rt] = h * a.group + (prow - node_of[rt] * a.group);
+    const int head = h * a.group + (prow - node_of[rt] * a.group);
     const char* qrow = static_cast<const char*>(p.q) +
-                       (int64_t(r.q0 + node_of[rt]) * p.q_stride_token + int64_t(head_of[rt]) * p.q_stride_head) * 2;
+                       (int64_t(r.q0 + node_of[rt]) * p.q_stride_token + int64_t(head) * p.q_stride_head) * 2;
     qscale[rt] = a.scale_log2;
     w4 v[KS];
 #pragma unroll
@@ -121,8 +121,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     }
     m_run[rt] = -INFINITY;
     l_run[rt] = 0.f;
-    slope[rt] = p.alibi_slopes ? p.alibi_slopes[head_of[rt]] * kPaLog2e : 0.f;
-    word[rt] = (p.mask_mode == 1 && p.mask_words == 1 && ok) ? p.tree_mask[r.q0 + node_of[rt]] : 0ull;
+    slope[rt] = p.alibi_slopes ? p.alibi_slopes[head] * kPaLog2e : 0.f;
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -198,38 +197,60 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
                                        (p.window_left < 0 || kb >= shift + k.n1 - p.window_left)));
     return kb + TK > (p.mask_mode == 1 ? min(r.kv_len, col0) : r.kv_len);
   };
+  // Infinities and NaN in V rows that a row does not see must not reach it (0 * inf):
+  // in tiles with hidden keys they are stored as zeros and marked, and the rows
+  // that see them get them from the marks.
+  auto take_out = [&](frag v, int st, int row, int gr) {
+    constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u;
+    uint32_t up = 0, dn = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = (v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+      const uint32_t bad = (x & kExp) == kExp ? 1u : 0u, nan = (x & 0x7fffu) > kExp ? 1u : 0u, neg = x >> 15;
+      up |= (bad & (nan | (neg ^ 1u))) << i;
+      dn |= (bad & (nan | neg)) << i;
+      if (bad) v[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
+    }
+    up_lds[st][row * (D / 8) + gr] = uint8_t(up);
+    dn_lds[st][row * (D / 8) + gr] = uint8_t(dn);
+    return v;
+  };
   auto store = [&](int st, int c) {
     char* kd = lds[st];
     char* vd = lds[st] + HALF;
-    // Infinities and NaN in V rows that a row does not see must not reach it
-    // (0 * inf): tiles with hidden keys that hold some are marked.
-    bool odd = false;
-    const bool look = KIND != kCacheInt8 && masked_tile(key_of(c));
+    frag vv[Q8 ? 2 * NL : NL];
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int row = j * RSTEP + prow0;
       if constexpr (!Q8) {
         *reinterpret_cast<w4*>(kd + row * RB + ((piece ^ (row & KSW)) << 4)) = kraw[j];
-        *reinterpret_cast<w4*>(vd + row * RB + ((piece ^ ((row & VSW) << 1)) << 4)) = vraw[j];
-        if (look) {
-          constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) odd |= (vraw[j][w] & kExp) == kExp || ((vraw[j][w] >> 16) & kExp) == kExp;
-        }
+        vv[j] = vraw[j];
       } else {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int gr = 2 * piece + e;
-          *reinterpret_cast<frag*>(kd + row * RB + ((gr ^ (row & KSW)) << 4)) = C::keys8(kraw[j][2 * e], kraw[j][2 * e + 1]);
-          *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = C::keys8(vraw[j][2 * e], vraw[j][2 * e + 1]);
-        }
-        if (KIND == kCacheE4M3 && look) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= ((vraw[j][w] >> (8 * e)) & 0x7fu) == 0x7fu;
+          *reinterpret_cast<frag*>(kd + row * RB + (((2 * piece + e) ^ (row & KSW)) << 4)) =
+              C::keys8(kraw[j][2 * e], kraw[j][2 * e + 1]);
+          vv[2 * j + e] = C::keys8(vraw[j][2 * e], vraw[j][2 * e + 1]);
         }
       }
+    }
+    if (KIND != kCacheInt8 && masked_tile(key_of(c))) {
+      constexpr uint32_t kExp = C::kBf16 ? 0x7f807f80u : 0x7c007c00u, kLow = C::kBf16 ? 0x00800080u : 0x04000400u;
+      uint32_t odd = 0;  // (an exponent of all ones carries into the sign's place)
+#pragma unroll
+      for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) odd |= (vv[j][w] & kExp) + kLow;
+      // (the marks of a tile are whole: every wave writes its part, whether it has some or not)
+#pragma unroll
+      for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j)
+        vv[j] = take_out(vv[j], st, (Q8 ? j >> 1 : j) * RSTEP + prow0, Q8 ? 2 * piece + (j & 1) : piece);
+      if (odd & 0x80008000u) strange_lds[st] = c + 1;
+    }
+#pragma unroll
+    for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j) {
+      const int row = (Q8 ? j >> 1 : j) * RSTEP + prow0, gr = Q8 ? 2 * piece + (j & 1) : piece;
+      *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = vv[j];
     }
     if constexpr (Q8 && PAGE16) {
       if (tid == 0) {
@@ -242,7 +263,6 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         scale_lds[st][1][tid >> 2] = vsc[0];
       }
     }
-    if (look && odd) strange_lds[st] = c + 1;
   };
 
   // Largest V scale so far: O holds sums of p * v * (scale / vref).
@@ -252,177 +272,182 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int e4 = r16 >> 2, q4 = r16 & 3;
   const int vkey = 4 * g + e4;
 
-  // One tile for this wave's first NR row tiles.
-  auto compute = [&](auto nr_tag, int st, int c) {
-    constexpr int NR = decltype(nr_tag)::value;
+  // One tile for this wave's row tiles, 32 keys at a time.
+  auto compute = [&](int st, int c) {
     const int kb = key_of(c);
     const char* kd = lds[st];
     const char* vd = lds[st] + HALF;
-    f32x4 acc[NR][4];
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-      for (int rt = 0; rt < NR; ++rt) acc[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const frag kf = *reinterpret_cast<const frag*>(kd + (kt * 16 + r16) * RB + (((ks * 4 + g) ^ (r16 & KSW)) << 4));
-#pragma unroll
-        for (int rt = 0; rt < NR; ++rt) acc[rt][kt] = C::mfma(kf, qf[rt][ks], acc[rt][kt]);
-      }
-    }
-    f32x4 ksk[PAGE16 ? 1 : 4], vsk[PAGE16 ? 1 : 4];  // scales of the 16-key tiles, or of the lane's keys
-    if constexpr (Q8) {
-#pragma unroll
-      for (int kt = 0; kt < (PAGE16 ? 1 : 4); ++kt) {
-        ksk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][0][PAGE16 ? 0 : kt * 16 + 4 * g]);
-        vsk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][1][PAGE16 ? 0 : kt * 16 + 4 * g]);
-      }
-      float top = vsk[0][0];
-#pragma unroll
-      for (int i = 1; i < (PAGE16 ? 4 : 16); ++i) top = fmaxf(top, vsk[i >> 2][i & 3]);
-      if constexpr (!PAGE16) top = groups_max(top);
-      if (__builtin_amdgcn_ballot_w64(top > vref) != 0) {
-        const float down = vref / top;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int t = 0; t < DT; ++t) o[rt][t] *= down;
-        vref = top;
-        vinv = 1.0f / top;
-      }
-    }
     const bool masked = masked_tile(kb);
-    frag pf[NR][2];
+    const bool strange = masked && KIND != kCacheInt8 && strange_lds[st] == c + 1;
 #pragma unroll
-    for (int rt = 0; rt < NR; ++rt) {
-      float sc[16];
+    for (int hh = 0; hh < 2; ++hh) {
+      f32x4 acc[RT][2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float f = qscale[rt];
-        if constexpr (Q8) f *= PAGE16 ? ksk[0][i >> 2] : ksk[PAGE16 ? 0 : i >> 2][i & 3];
-        sc[i] = acc[rt][i >> 2][i & 3] * f;
-      }
-      if (p.soft_cap > 0.f) {
-        // cap * tanh(y / cap) = cap * (1 - 2 / (1 + e^(2 y / cap))), to powers of two
+      for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(sc[i] * a.cap_in);
-          sc[i] = __builtin_fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(1.f + e), a.cap_out);
+        for (int rt = 0; rt < RT; ++rt) acc[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const frag kf = *reinterpret_cast<const frag*>(kd + (hh * 32 + kt * 16 + r16) * RB +
+                                                         (((ks * 4 + g) ^ (r16 & KSW)) << 4));
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt][kt] = C::mfma(kf, qf[rt][ks], acc[rt][kt]);
         }
       }
-      const int qpos = shift + node_of[rt];
-      const int key0 = kb + 4 * g;
-      if (p.alibi_slopes != nullptr) {
-        const float away = float(qpos - key0);
+      f32x4 ksk[2], vsk[2];  // scales of the lane's keys (by 16-key tile: the first element)
+      if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          sc[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), sc[i]);
-      }
-      if (masked) {
-        uint64_t w = word[rt];
-        int w0 = col0;
-        if (p.mask_mode == 1 && p.mask_words > 1) {
-          // one word for each 64 keys, and a tile is one of them
-          const int idx = (kb >> 6) - (col0 >> 6);
-          w = idx < 0 ? ~0ull
-                      : (idx < p.mask_words && (wave + 4 * rt) * 16 + r16 < rows
-                             ? p.tree_mask[int64_t(r.q0 + node_of[rt]) * p.mask_words + idx] : 0ull);
-          w0 = kb;
-        }
-        const int wlo = p.window_left >= 0 ? qpos - p.window_left : 0;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          const int at = key0 + kt * 16;
-          uint32_t vis = below4(at, r.kv_len);
-          if (p.mask_mode == 2) {
-            vis &= (below4(at, qpos + 1) & ~below4(at, wlo)) | below4(at, k.prefix);
-          } else if (p.mask_mode == 1) {
-            const int off = at - w0;  // the lane's keys in the word; those before it are the prefix
-            const int pre = min(max(-off, 0), 4);
-            const uint32_t up = off >= 0 && off < 64 ? uint32_t(w >> (off & 63)) : 0u;
-            const uint32_t down = uint32_t(w << pre) | ((1u << pre) - 1u);
-            vis &= off >= 0 ? up : down;
+        for (int kt = 0; kt < 2; ++kt) {
+          if constexpr (PAGE16) {
+            ksk[kt][0] = scale_lds[st][0][hh * 2 + kt];
+            vsk[kt][0] = scale_lds[st][1][hh * 2 + kt];
+          } else {
+            ksk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][0][hh * 32 + kt * 16 + 4 * g]);
+            vsk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][1][hh * 32 + kt * 16 + 4 * g]);
           }
+        }
+        float top = fmaxf(vsk[0][0], vsk[1][0]);
+        if constexpr (!PAGE16) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[kt * 4 + i] = (vis >> i) & 1u ? sc[kt * 4 + i] : -INFINITY;
+          for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(vsk[0][i], vsk[1][i]));
+          top = groups_max(top);
+        }
+        if (__builtin_amdgcn_ballot_w64(top > vref) != 0) {
+          const float down = vref / top;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[rt][t] *= down;
+          vref = top;
+          vinv = 1.0f / top;
         }
       }
-      float mx = sc[0];
+      frag pf[RT];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = pa_max(mx, sc[i]);
-      if (__builtin_amdgcn_ballot_w64(mx > m_run[rt] + kPaLazyLog2) != 0) {
-        const float top = groups_max(mx);
-        const bool grow = top > m_run[rt] + kPaLazyLog2;  // (a row's results do not depend on its neighbours)
-        const float m_new = grow ? top : m_run[rt];
-        const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[rt] - m_new) : 1.f;
-        l_run[rt] *= alpha;
+      for (int rt = 0; rt < RT; ++rt) {
+        const int qpos = shift + node_of[rt];
+        const int key0 = kb + hh * 32 + 4 * g;
+        // x: scores to powers of two; without a cap, a bias or hidden keys the factor (not
+        // negative there) is left to the exponent
+        float x[8], f[PAGE16 || !Q8 ? 2 : 8];
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[rt][t] *= alpha;
-        m_run[rt] = m_new;
-      }
-      const float m = m_run[rt] == -INFINITY ? 0.f : m_run[rt];
+        for (int i = 0; i < 8; ++i) x[i] = acc[rt][i >> 2][i & 3];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        float e[4];
+        for (int i = 0; i < (PAGE16 || !Q8 ? 2 : 8); ++i)
+          f[i] = !Q8 ? qscale[rt] : qscale[rt] * (PAGE16 ? ksk[i][0] : ksk[i >> 2][i & 3]);
+        const bool plain = p.soft_cap == 0.f && p.alibi_slopes == nullptr && !masked && p.sm_scale >= 0.f;
+        if (!plain) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(sc[kt * 4 + i] - m);
-          l_run[rt] += e[i];
-          if constexpr (Q8) e[i] *= (PAGE16 ? vsk[0][kt] : vsk[PAGE16 ? 0 : kt][i]) * vinv;
-        }
-        pf[rt][kt >> 1][(kt & 1) * 2] = C::pack(e[0], e[1]);
-        pf[rt][kt >> 1][(kt & 1) * 2 + 1] = C::pack(e[2], e[3]);
-      }
-    }
-    // V^T's operand of dim tile t and the keys 32 hh .. + 31 of the tile
-    auto v_frag = [&](int t, int hh) {
-      const char* at = vd + (32 * hh + vkey) * RB + (((2 * t + (q4 >> 1)) ^ ((vkey & VSW) << 1)) << 4) + ((q4 & 1) << 3);
-      const w2 x = read_tr16(at), y = read_tr16(at + 16 * RB);
-      return frag{x[0], x[1], y[0], y[1]};
-    };
-    if (!(masked && KIND != kCacheInt8 && strange_lds[st] == c + 1)) {
+          for (int i = 0; i < 8; ++i) x[i] *= f[PAGE16 || !Q8 ? i >> 2 : i];
+          if (p.soft_cap > 0.f) {
+            // cap * tanh(y / cap) = cap * (1 - 2 / (1 + e^(2 y / cap))), to powers of two
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const frag vf = v_frag(t, hh);
-#pragma unroll
-          for (int rt = 0; rt < NR; ++rt) o[rt][t] = C::mfma(vf, pf[rt][hh], o[rt][t]);
-        }
-    } else {
-      // finite values as they are; where a row that sees the key has an infinity or
-      // NaN, its sum becomes one
-      constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u, kOne = C::kBf16 ? 0x3f80u : 0x3c00u;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          const frag vf = v_frag(t, hh);
-          frag fine, up, dn;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            fine[j] = up[j] = dn[j] = 0;
-#pragma unroll
-            for (int hw = 0; hw < 2; ++hw) {
-              const uint32_t v = (vf[j] >> (16 * hw)) & 0xffffu;
-              const bool bad = (v & kExp) == kExp, nan = (v & 0x7fffu) > kExp;
-              fine[j] |= (bad ? 0u : v) << (16 * hw);
-              up[j] |= (bad && (nan || v == kExp) ? kOne : 0u) << (16 * hw);
-              dn[j] |= (bad && (nan || v != kExp) ? kOne : 0u) << (16 * hw);
+            for (int i = 0; i < 8; ++i) {
+              const float e = __builtin_amdgcn_exp2f(x[i] * a.cap_in);
+              x[i] = __builtin_fmaf(-2.f * a.cap_out, __builtin_amdgcn_rcpf(1.f + e), a.cap_out);
             }
           }
+          if (p.alibi_slopes != nullptr) {
+            const float away = float(qpos - key0);
 #pragma unroll
-          for (int rt = 0; rt < NR; ++rt) {
+            for (int i = 0; i < 8; ++i)
+              x[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), x[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < (PAGE16 || !Q8 ? 2 : 8); ++i) f[i] = 1.f;
+        }
+        if (masked) {
+          uint64_t w = 0;
+          int w0 = col0;
+          if (p.mask_mode == 1) {
+            // one word of the tree's columns, or one for each 64 keys (a tile is one of them)
+            const int idx = p.mask_words > 1 ? (kb >> 6) - (col0 >> 6) : 0;
+            if (idx >= 0 && idx < p.mask_words) w = p.tree_mask[int64_t(r.q0 + node_of[rt]) * p.mask_words + idx];
+            if (idx < 0) w = ~0ull;
+            if (p.mask_words > 1) w0 = kb;
+          }
+          const int wlo = p.window_left >= 0 ? qpos - p.window_left : 0;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            const int at = key0 + kt * 16;
+            uint32_t vis = below4(at, r.kv_len);
+            if (p.mask_mode == 2) {
+              vis &= (below4(at, qpos + 1) & ~below4(at, wlo)) | below4(at, k.prefix);
+            } else if (p.mask_mode == 1) {
+              const int off = at - w0;  // the lane's keys in the word; those before it are the prefix
+              const int pre = min(max(-off, 0), 4);
+              const uint32_t up = off >= 0 && off < 64 ? uint32_t(w >> (off & 63)) : 0u;
+              const uint32_t down = uint32_t(w << pre) | ((1u << pre) - 1u);
+              vis &= off >= 0 ? up : down;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[kt * 4 + i] = (vis >> i) & 1u ? x[kt * 4 + i] : -INFINITY;
+          }
+        }
+        float mx;
+        if constexpr (PAGE16 || !Q8) {
+          mx = pa_max(pa_max(pa_max(x[0], x[1]), pa_max(x[2], x[3])) * f[0],
+                      pa_max(pa_max(x[4], x[5]), pa_max(x[6], x[7])) * f[1]);
+        } else {
+          mx = x[0] * f[0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) mx = pa_max(mx, x[i] * f[i]);
+        }
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[rt] + kPaLazyLog2) != 0) {
+          const float top = groups_max(mx);
+          const bool grow = top > m_run[rt] + kPaLazyLog2;  // (a row's results do not depend on its neighbours)
+          const float m_new = grow ? top : m_run[rt];
+          const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[rt] - m_new) : 1.f;
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) o[rt][t] *= alpha;
+          m_run[rt] = m_new;
+        }
+        const float m = m_run[rt] == -INFINITY ? 0.f : m_run[rt];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          float e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kt * 4 + i], f[PAGE16 || !Q8 ? kt : kt * 4 + i], -m));
+            l_run[rt] += e[i];
+            if constexpr (Q8) e[i] *= vsk[kt][PAGE16 ? 0 : i] * vinv;
+          }
+          pf[rt][kt * 2] = C::pack(e[0], e[1]);
+          pf[rt][kt * 2 + 1] = C::pack(e[2], e[3]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        // V^T's operand of dim tile t
+        const char* at = vd + (32 * hh + vkey) * RB + (((2 * t + (q4 >> 1)) ^ ((vkey & VSW) << 1)) << 4) + ((q4 & 1) << 3);
+        const w2 lo = read_tr16(at), hi = read_tr16(at + 16 * RB);
+        const frag vf = frag{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf, pf[rt], o[rt][t]);
+      }
+      if (strange) {
+        // Where a row sees an infinity or NaN, its sum becomes one: a product with the
+        // marks is zero for the rows that do not.
+        constexpr uint32_t kOne = C::kBf16 ? 0x3f80u : 0x3c00u;
+        constexpr float kHuge = 3e38f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          frag up = frag{0, 0, 0, 0}, dn = up;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int byte = (32 * hh + 16 * (j >> 2) + 4 * g + (j & 3)) * (D / 8) + 2 * t + (r16 >> 3);
+            up[j >> 1] |= ((uint32_t(up_lds[st][byte]) >> (r16 & 7)) & 1u) * (kOne << (16 * (j & 1)));
+            dn[j >> 1] |= ((uint32_t(dn_lds[st][byte]) >> (r16 & 7)) & 1u) * (kOne << (16 * (j & 1)));
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
             const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-            o[rt][t] = C::mfma(fine, pf[rt][hh], o[rt][t]);
-            const f32x4 plus = C::mfma(up, pf[rt][hh], zero), minus = C::mfma(dn, pf[rt][hh], zero);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (plus[i] > 0.f) o[rt][t][i] += INFINITY;
-              if (minus[i] > 0.f) o[rt][t][i] -= INFINITY;
-            }
+            const f32x4 plus = C::mfma(up, pf[rt], zero), minus = C::mfma(dn, pf[rt], zero);
+            o[rt][t] += plus * kHuge * kHuge - minus * kHuge * kHuge;
           }
         }
+      }
     }
   };
 
@@ -445,10 +470,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       // before the last barrier; then the one behind it is asked for
       if (c + 1 < c1) store(st ^ 1, c + 1);
       if (c + 2 < c1) load(c + 2);
-      if (nrt == 1) compute(std::integral_constant<int, 1>{}, st, c);
-      if constexpr (RT == 2) {
-        if (nrt == 2) compute(std::integral_constant<int, 2>{}, st, c);
-      }
+      if (computes) compute(st, c);
       lds_barrier();
     }
   }
@@ -470,8 +492,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(ws + prow * D + t * 16 + 4 * g) = o[rt][t] * inv;
       if (g == 0) ws[nrows * D + prow] = lse2;
     } else {
+      const int head = h * a.group + (row_start + lr - node_of[rt] * a.group);
       char* out = static_cast<char*>(p.out) + (int64_t(r.q0 + node_of[rt]) * p.out_stride_token +
-                                               int64_t(head_of[rt]) * p.out_stride_head) * 2;
+                                               int64_t(head) * p.out_stride_head) * 2;
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
         const f32x4 x = o[rt][t] * inv;
@@ -479,7 +502,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
             bf16 ? w2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])} : w2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])};
       }
       if (p.lse != nullptr && g == 0)
-        p.lse[int64_t(r.q0 + node_of[rt]) * p.num_qo_heads + head_of[rt]] = lse2 * kPaLn2;
+        p.lse[int64_t(r.q0 + node_of[rt]) * p.num_qo_heads + head] = lse2 * kPaLn2;
     }
   }
 }

@@ -32,11 +32,17 @@ import torch
 from . import _lib
 from .tree_attention import _host_lists
 
-# Most packed query rows (query token * group + head of the group) of a workgroup.
+# Most packed query rows (query token * group + head of the group) of a workgroup:
+# of the decode kernel, and of the kernel for several tokens with one and with two
+# row tiles a wave.
 DECODE_ROWS = 16
-BLOCK_ROWS = 128
+BLOCK_ROWS = 64
+WIDE_BLOCK_ROWS = 128
+# Requests of more packed rows than this take the wide blocks.
+MAX_NARROW_ROWS = 192
 # Workgroups to aim for when the keys are split, and the least keys of a split.
-TARGET_WORKGROUPS = 1024
+DECODE_WORKGROUPS = 1024
+BLOCK_WORKGROUPS = 512
 MIN_SPLIT_KEYS = 256
 MAX_SPLITS = 256
 
@@ -51,16 +57,20 @@ def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_l
     """(single token?, rows of a block, row blocks, splits, keys per split) of a call.
 
     One query token per request takes the decode kernel with blocks of 16 packed
-    rows.  More take equal blocks of up to BLOCK_ROWS.  Keys are split until about
-    TARGET_WORKGROUPS workgroups are there, in splits of at least MIN_SPLIT_KEYS;
-    a request shorter than ``max_kv_len`` takes fewer splits of the same size."""
+    rows, more take equal blocks.  Keys are split until about as many workgroups are
+    there as the device holds at once, in splits of at least MIN_SPLIT_KEYS; a
+    request shorter than ``max_kv_len`` takes fewer splits of the same size."""
     single = max_q_len <= 1 and not tree
     rows = max(1, max_q_len * group)
-    blocks = -(-rows // (DECODE_ROWS if single else BLOCK_ROWS))
-    block_rows = DECODE_ROWS if single else 16 * -(-rows // (16 * blocks))
+    if single:
+        block_rows, target = DECODE_ROWS, DECODE_WORKGROUPS
+        blocks = -(-rows // DECODE_ROWS)
+    else:
+        blocks = -(-rows // (BLOCK_ROWS if rows <= MAX_NARROW_ROWS else WIDE_BLOCK_ROWS))
+        block_rows, target = 16 * -(-rows // (16 * blocks)), BLOCK_WORKGROUPS
     items = batch * kv_heads * blocks
     most = min(MAX_SPLITS, max(1, -(-max_kv_len // MIN_SPLIT_KEYS)))
-    splits = max(1, min(most, -(-TARGET_WORKGROUPS // items)))
+    splits = max(1, min(most, target // items))
     keys = max(64, -(-max_kv_len // splits))
     keys = -(-keys // 64) * 64
     return single, block_rows, blocks, max(1, -(-max_kv_len // keys)), keys

@@ -344,3 +344,13 @@ def test_extreme_scales_and_queries(dev):
     big["scales"][:, 0] *= 2.0 ** -110
     big["q"] = (s["q"].float() * 2.0 ** 110).to(torch.bfloat16)
     check(big, call(dev, big))
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=str)
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-30])
+def test_other_score_scales(dev, cache, scale):
+    """sm_scale negative, zero and tiny: hidden keys stay hidden, the rest is as defined."""
+    s = build(81, [1, 30], [100, 90], cache=cache)
+    check(s, call(dev, s, causal=True, sm_scale=scale), causal=True, sm_scale=scale)
+    one = build(82, [1, 1], [100, 70], cache=cache)
+    check(one, call(dev, one, causal=True, window_left=40, sm_scale=scale), causal=True, window_left=40, sm_scale=scale)
