@@ -79,7 +79,10 @@ extern "C" int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream) {
   a.cap_in = p.soft_cap > 0.f ? 2.f / p.soft_cap : 0.f;
   a.cap_out = p.soft_cap * kPaLog2e;
   a.group = p.num_qo_heads / p.num_kv_heads;
-  a.page_shift = ilog2_exact(p.page_size);
+  int bits = 0;
+  while ((int64_t(1) << bits) < p.page_size) ++bits;
+  a.page_magic = uint32_t(((uint64_t(1) << (31 + bits)) + p.page_size - 1) / p.page_size);
+  a.page_bits = 31 + bits;
   return p.cache == ATLAS_CACHE_16BIT ? launch_paged_attn_16bit(a, static_cast<hipStream_t>(stream))
                                       : launch_paged_attn_q8(a, static_cast<hipStream_t>(stream));
 }

@@ -37,7 +37,9 @@ struct PagedAttnArgs {
   float cap_in;      // soft cap: 2 * log2(e) * sm_scale / cap
   float cap_out;     // cap * log2(e)
   int group;
-  int page_shift;  // log2(page_size), or -1
+  // key / page_size = key * page_magic >> page_bits for keys below 2^31
+  uint32_t page_magic;
+  int page_bits;
 };
 
 int launch_paged_attn_16bit(const PagedAttnArgs& a, hipStream_t stream);
@@ -254,61 +256,48 @@ __device__ __forceinline__ float q_to_f16(const float (&f)[KS][8], w4 (&q)[KS]) 
   return __uint_as_float(uint32_t(127 + e) << 23);
 }
 
-// The request's pages as a wave reads them, 64 at a time: lane l holds the id (and
-// its scales) of page slot win * 64 + l, so that a tile's page costs a readlane
-// and no memory access waits behind another in the key loop.  Two windows are held;
-// entering the second asks for the one behind it.
-template <bool Q8>
-struct PageWindow {
+__device__ __forceinline__ int slot_of(const PagedAttnArgs& a, int key) {
+  return int((uint64_t(uint32_t(key)) * a.page_magic) >> a.page_bits);
+}
+
+// Pages of the 16-key tiles of one step, for page sizes that are multiples of 16.
+// Lane l holds what belongs to tile l % KT: its page id, read two steps before the
+// step's rows are asked for, and its scales (K's in lanes of even l / KT, V's in the others), read one
+// step before.  The tiles' values come back by readlane, and no memory access
+// of the key loop waits for another.
+template <bool Q8, int KT>
+struct TilePages {
   const int32_t* ids;  // the request's page ids
   const float* scales;
-  int64_t scale_page, scale_kv;
+  int64_t scale_page;
   int64_t last_id;  // ids are clamped to [0, last_id]
-  int last_slot;    // slots are clamped to it
-  int lane, win;
-  int id0, id1;
-  float ks0, ks1, vs0, vs1;
 
-  __device__ __forceinline__ void fetch(int w, int& id, float& ks, float& vs) const {
-    int64_t x = ids[min(w * 64 + lane, last_slot)];
-    x = x < 0 ? 0 : (x > last_id ? last_id : x);
-    id = int(x);
-    if constexpr (Q8) {
-      const float* s = scales + x * scale_page;
-      ks = s[0];
-      vs = s[scale_kv];
-    }
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const Request& r, int h, int lane) {
+    ids = a.p.kv_indices + r.pt;
+    if constexpr (Q8)
+      scales = a.p.kv_scales + int64_t(h) * a.p.scale_stride_head + ((lane / KT) & 1) * a.p.scale_stride_kv;
+    scale_page = a.p.scale_stride_page;
+    last_id = a.p.num_pages - 1;
   }
-  __device__ __forceinline__ void begin(int slot) {
-    win = slot >> 6;
-    fetch(win, id0, ks0, vs0);
-    fetch(win + 1, id1, ks1, vs1);
+  // First key of the lane's tile of the step at kb, on a tile that holds a key of [lo, hi]
+  static __device__ __forceinline__ int tile_key(int kb, int kt, int lo, int hi) {
+    return min(max(kb + kt * 16, lo & ~15), hi & ~15);
   }
-  // Makes slots up to `slot` readable (slots only grow, but for a new start).
-  __device__ __forceinline__ void reach(int slot) {
-    const int w = slot >> 6;
-    if (w <= win + 1) return;
-    if (w == win + 2) {
-      win = w - 1;
-      id0 = id1;
-      ks0 = ks1;
-      vs0 = vs1;
-      fetch(w, id1, ks1, vs1);
-    } else {
-      begin(slot);
-    }
+  __device__ __forceinline__ int read_id(const PagedAttnArgs& a, int kb, int lo, int hi, int lane) const {
+    return ids[slot_of(a, tile_key(kb, lane & (KT - 1), lo, hi))];
   }
-  __device__ __forceinline__ int id(int slot) const {
-    const int l = slot & 63;
-    return (slot >> 6) == win ? __builtin_amdgcn_readlane(id0, l) : __builtin_amdgcn_readlane(id1, l);
+  __device__ __forceinline__ int64_t valid(int id) const {
+    const int64_t x = id;
+    return x < 0 ? 0 : (x > last_id ? last_id : x);
   }
-  __device__ __forceinline__ float lane_float(float a, float b, int slot) const {
-    const int l = slot & 63;
-    return __uint_as_float((slot >> 6) == win ? __builtin_amdgcn_readlane(__float_as_uint(a), l)
-                                              : __builtin_amdgcn_readlane(__float_as_uint(b), l));
+  __device__ __forceinline__ float read_scale(int id) const {
+    if constexpr (Q8) return scales[valid(id) * scale_page];
+    else return 0.f;
   }
-  __device__ __forceinline__ float k_scale(int slot) const { return lane_float(ks0, ks1, slot); }
-  __device__ __forceinline__ float v_scale(int slot) const { return lane_float(vs0, vs1, slot); }
+  static __device__ __forceinline__ int tile_id(int v, int kt) { return __builtin_amdgcn_readlane(v, kt); }
+  static __device__ __forceinline__ float tile_scale(float v, int kv, int kt) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), kv * KT + kt));
+  }
 };
 
 // Joins the splits of a row block: one wave per row, its lanes over the dims.

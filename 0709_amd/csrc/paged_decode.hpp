@@ -121,16 +121,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
   const char* kbase = static_cast<const char*>(p.kv) + int64_t(h) * p.head_stride;
   const char* vbase = kbase + p.v_offset;
   const int ts = int(p.token_stride);
-  PageWindow<Q8> pages;
-  pages.ids = p.kv_indices + r.pt;
-  pages.scales = Q8 ? p.kv_scales + int64_t(h) * p.scale_stride_head : nullptr;
-  pages.scale_page = p.scale_stride_page;
-  pages.scale_kv = p.scale_stride_kv;
-  pages.last_id = p.num_pages - 1;
-  pages.lane = lane;
   const int page_size = p.page_size;
-  auto slot_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / page_size; };
-  pages.last_slot = k.hi > 0 ? slot_of(max(k.hi, k.prefix) - 1) : 0;
+  TilePages<Q8, KT> pages;
+  pages.begin(a, r, h, lane);
 
   struct Raw {
     uint32_t k[KT][KL * 4];
@@ -142,75 +135,70 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
     const int c = s / SUB;
     return (c < k.ca ? c : c - k.ca + k.cb) * kChunk + (s % SUB) * CK;
   };
+  auto bounds = [&](int s, int& lo, int& hi) {
+    const bool first = s < k.ca * SUB;
+    lo = first ? 0 : k.lo;
+    hi = (first ? k.prefix : k.hi) - 1;
+  };
+  auto read_id = [&](int s) {
+    int lo, hi;
+    bounds(s, lo, hi);
+    return pages.read_id(a, key_of(s), lo, hi, lane);
+  };
   // lane offsets of a tile's rows
   const uint32_t k_lane = uint32_t(r16 * ts + g * 16), v_lane = uint32_t(4 * g * ts + r16 * VB);
   // Keys outside [lo, hi) of the step's part repeat its nearest key, so that
   // every load falls on a row that is there.
-  auto load = [&](Raw& x, int s) {
+  auto load = [&](Raw& x, int s, int id, float scale) {
     const int kb = key_of(s);
-    const bool first = s < k.ca * SUB;
-    const int lo = first ? 0 : k.lo;
-    const int hi = (first ? k.prefix : k.hi) - 1;
+    int lo, hi;
+    bounds(s, lo, hi);
     if constexpr (PAGE16) {
-      uint32_t ko[KT], vo[KT][4];
-      int slot[KT];
-      if (kb >= lo && kb + CK <= hi + 1) {
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          slot[kt] = slot_of(kb + kt * 16);
-          const uint32_t at = uint32_t(kb + kt * 16 - slot[kt] * page_size) * uint32_t(ts);
-          ko[kt] = k_lane + at;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vo[kt][i] = v_lane + at + uint32_t(i * ts);
-        }
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const int t0 = kb + kt * 16;
-          slot[kt] = slot_of(min(max(t0, lo & ~15), hi & ~15));
-          const int start = slot[kt] * page_size;
-          ko[kt] = uint32_t((min(max(t0 + r16, lo), hi) - start) * ts + g * 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            vo[kt][i] = uint32_t((min(max(t0 + 4 * g + i, lo), hi) - start) * ts + r16 * VB);
-        }
-      }
-      pages.reach(slot[KT - 1]);
+      const bool whole = kb >= lo && kb + CK <= hi + 1;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const int64_t at = int64_t(pages.id(slot[kt])) * p.page_stride;
-        const char* kp = kbase + at;
-        const char* vp = vbase + at;
+        const int tile = TilePages<Q8, KT>::tile_key(kb, kt, lo, hi);
+        const int64_t at = pages.valid(TilePages<Q8, KT>::tile_id(id, kt)) * p.page_stride;
+        // the tile's first row; then lane offsets from it
+        const int64_t row0 = at + int64_t(tile - slot_of(a, tile) * page_size) * ts;
+        const char* kp = kbase + row0;
+        const char* vp = vbase + row0;
+        uint32_t ko = k_lane, vo[4];
 #pragma unroll
-        for (int j = 0; j < KL; ++j) load_words<16>(kp + (ko[kt] + j * 64), &x.k[kt][4 * j]);
+        for (int i = 0; i < 4; ++i) vo[i] = v_lane + uint32_t(i * ts);
+        if (!whole) {
+          const int t0 = kb + kt * 16;
+          ko = uint32_t((min(max(t0 + r16, lo), hi) - tile) * ts + g * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) load_words<VB>(vp + vo[kt][i], x.v[kt][i]);
+          for (int i = 0; i < 4; ++i) vo[i] = uint32_t((min(max(t0 + 4 * g + i, lo), hi) - tile) * ts + r16 * VB);
+        }
+#pragma unroll
+        for (int j = 0; j < KL; ++j) load_words<16>(kp + (ko + j * 64), &x.k[kt][4 * j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_words<VB>(vp + vo[i], x.v[kt][i]);
         if constexpr (Q8) {
-          x.ks[kt] = pages.k_scale(slot[kt]);
-          x.vs[kt] = pages.v_scale(slot[kt]);
+          x.ks[kt] = TilePages<Q8, KT>::tile_scale(scale, 0, kt);
+          x.vs[kt] = TilePages<Q8, KT>::tile_scale(scale, 1, kt);
         }
       }
     } else {
-      auto page_of = [&](int slot) -> int64_t {
-        const int64_t id = pages.ids[slot];
-        return id < 0 ? 0 : (id > pages.last_id ? pages.last_id : id);
-      };
+      auto page_of = [&](int slot) { return pages.valid(pages.ids[slot]); };
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const int t0 = kb + kt * 16;
         const int key = min(max(t0 + r16, lo), hi);
-        const int slot = slot_of(key);
+        const int slot = slot_of(a, key);
         const char* kp = kbase + page_of(slot) * p.page_stride + int64_t(key - slot * page_size) * ts;
 #pragma unroll
         for (int j = 0; j < KL; ++j) load_words<16>(kp + j * 64 + g * 16, &x.k[kt][4 * j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int vk = min(max(t0 + 4 * g + i, lo), hi);
-          const int vslot = slot_of(vk);
+          const int vslot = slot_of(a, vk);
           const int64_t page = page_of(vslot);
           load_words<VB>(vbase + page * p.page_stride + int64_t(vk - vslot * page_size) * ts + r16 * VB, x.v[kt][i]);
           if constexpr (Q8) {
-            const float* sc = pages.scales + page * p.scale_stride_page;
+            const float* sc = p.kv_scales + int64_t(h) * p.scale_stride_head + page * p.scale_stride_page;
             x.ks[kt * 4 + i] = sc[0];
             x.vs[kt * 4 + i] = sc[p.scale_stride_kv];
           }
@@ -317,22 +305,37 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
   };
 
   if (s0 < s1) {
-    if constexpr (PAGE16) {
-      const bool first = s0 < k.ca * SUB;
-      pages.begin(slot_of(min(max(key_of(s0), first ? 0 : k.lo), (first ? k.prefix : k.hi) - 1)));
-    }
-    // The next step is in flight while this one is computed; the last one is asked
+    // The next step's rows, the scales of the one behind it and the page ids of the
+    // third are in flight while a step is computed; past the last step it is asked
     // for again rather than branched around, so the waits stay exact.
+    auto at = [&](int s) { return min(s, s1 - 1); };
+    int id0 = 0, id1 = 0, id2 = 0;
+    float sc0 = 0.f, sc1 = 0.f;
+    if constexpr (PAGE16) {
+      id0 = read_id(s0);
+      id1 = read_id(at(s0 + 1));
+      id2 = read_id(at(s0 + 2));
+      sc0 = pages.read_scale(id0);
+      sc1 = pages.read_scale(id1);
+    }
     Raw x, y;
-    load(x, s0);
+    load(x, s0, id0, sc0);
     int s = s0;
-    while (true) {
-      load(y, min(s + 1, s1 - 1));
-      compute(x, s);
-      if (++s >= s1) break;
-      load(x, min(s + 1, s1 - 1));
-      compute(y, s);
-      if (++s >= s1) break;
+    auto step = [&](Raw& cur, Raw& next) {
+      int id3 = 0;
+      float sc2 = 0.f;
+      if constexpr (PAGE16) {
+        id3 = read_id(at(s + 3));
+        sc2 = pages.read_scale(id2);
+      }
+      load(next, at(s + 1), id1, sc1);
+      compute(cur, s);
+      id1 = id2;
+      id2 = id3;
+      sc1 = sc2;
+      return ++s < s1;
+    };
+    while (step(x, y) && step(y, x)) {
     }
   }
 

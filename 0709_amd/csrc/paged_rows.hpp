@@ -131,71 +131,62 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const char* vbase = kbase + p.v_offset;
   const int ts = int(p.token_stride);
   const int page_size = p.page_size;
-  auto slot_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / page_size; };
-  PageWindow<Q8> pages;
-  pages.ids = p.kv_indices + r.pt;
-  pages.scales = Q8 ? p.kv_scales + int64_t(h) * p.scale_stride_head : nullptr;
-  pages.scale_page = p.scale_stride_page;
-  pages.scale_kv = p.scale_stride_kv;
-  pages.last_id = p.num_pages - 1;
-  pages.lane = lane;
-  pages.last_slot = k.hi > 0 ? slot_of(max(k.hi, k.prefix) - 1) : 0;
+  TilePages<Q8, 4> pages;
+  pages.begin(a, r, h, lane);
 
   auto key_of = [&](int c) { return (c < k.ca ? c : c - k.ca + k.cb) * TK; };
   auto bounds = [&](int c, int& lo, int& hi) {
     lo = c < k.ca ? 0 : k.lo;
     hi = (c < k.ca ? k.prefix : k.hi) - 1;
   };
+  auto read_id = [&](int c) {
+    int lo, hi;
+    bounds(c, lo, hi);
+    return pages.read_id(a, key_of(c), lo, hi, lane);
+  };
   // Piece j of a thread: row (j * 256 + tid) / GG of the tile, piece tid % GG of it.
   const int piece = tid % GG, prow0 = tid / GG;
   constexpr int RSTEP = kPaThreads / GG;  // rows between a thread's pieces
   w4 kraw[NL], vraw[NL];
-  float ksc[PAGE16 ? 4 : 1], vsc[PAGE16 ? 4 : 1];  // scales of its 16-key tiles, or of key tid / 4
+  float tile_scales = 0.f;       // scales of the tile in kraw / vraw, as read
+  float ksc = 0.f, vsc = 0.f;    // other page sizes: those of key tid / 4
   // Keys outside [lo, hi) of the tile's part repeat its nearest key.
-  auto load = [&](int c) {
+  auto load = [&](int c, int id, float scale) {
     const int kb = key_of(c);
     int lo, hi;
     bounds(c, lo, hi);
-    if constexpr (PAGE16) pages.reach(slot_of(min(max(kb + TK - 16, lo & ~15), hi & ~15)));
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
-      int64_t at;
       if constexpr (PAGE16) {
         // (a wave's rows of one piece lie in one 16-key tile)
-        const int t0 = kb + ((j * RSTEP + wave * (64 / GG)) & ~15);
-        const int slot = slot_of(min(max(t0, lo & ~15), hi & ~15));
-        at = int64_t(pages.id(slot)) * p.page_stride + uint32_t((key - slot * page_size) * ts + piece * 16);
+        const int kt = (j * RSTEP + wave * (64 / GG)) >> 4;
+        const int tile = TilePages<Q8, 4>::tile_key(kb, kt, lo, hi);
+        const int64_t row0 = pages.valid(__builtin_amdgcn_readlane(id, kt)) * p.page_stride +
+                             int64_t(tile - slot_of(a, tile) * page_size) * ts;
+        const uint32_t off = uint32_t((key - tile) * ts + piece * 16);
+        kraw[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
+        vraw[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);
       } else {
-        const int slot = slot_of(key);
-        const int64_t id = pages.ids[slot];
-        at = (id < 0 ? 0 : (id > pages.last_id ? pages.last_id : id)) * p.page_stride +
-             int64_t(key - slot * page_size) * ts + piece * 16;
+        const int slot = slot_of(a, key);
+        const int64_t at = pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts + piece * 16;
+        kraw[j] = *reinterpret_cast<const w4*>(kbase + at);
+        vraw[j] = *reinterpret_cast<const w4*>(vbase + at);
       }
-      kraw[j] = *reinterpret_cast<const w4*>(kbase + at);
-      vraw[j] = *reinterpret_cast<const w4*>(vbase + at);
     }
-    if constexpr (Q8 && PAGE16) {
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        const int slot = slot_of(min(max(kb + kt * 16, lo & ~15), hi & ~15));
-        ksc[kt] = pages.k_scale(slot);
-        vsc[kt] = pages.v_scale(slot);
-      }
-    } else if constexpr (Q8) {
-      const int slot = slot_of(min(max(kb + (tid >> 2), lo), hi));
-      const int64_t id = pages.ids[slot];
-      const float* s = pages.scales + (id < 0 ? 0 : (id > pages.last_id ? pages.last_id : id)) * p.scale_stride_page;
-      ksc[0] = s[0];
-      vsc[0] = s[p.scale_stride_kv];
+    tile_scales = scale;
+    if constexpr (Q8 && !PAGE16) {
+      const int slot = slot_of(a, min(max(kb + (tid >> 2), lo), hi));
+      const float* s = p.kv_scales + int64_t(h) * p.scale_stride_head + pages.valid(pages.ids[slot]) * p.scale_stride_page;
+      ksc = s[0];
+      vsc = s[p.scale_stride_kv];
     }
   };
   // Does some key of tile c hide from some row?
+  const int plain_hi = p.mask_mode == 2 ? shift + k.n0 + 1 : (p.mask_mode == 1 ? min(r.kv_len, col0) : r.kv_len);
+  const int plain_lo = p.mask_mode == 2 && p.window_left >= 0 ? shift + k.n1 - p.window_left : 0;
   auto masked_tile = [&](int kb) {
-    if (p.mask_mode == 2)
-      return !(kb + TK <= k.prefix || (kb + TK <= shift + k.n0 + 1 &&
-                                       (p.window_left < 0 || kb >= shift + k.n1 - p.window_left)));
-    return kb + TK > (p.mask_mode == 1 ? min(r.kv_len, col0) : r.kv_len);
+    return ((kb + TK > plain_hi) | (kb < plain_lo)) & (kb + TK > k.prefix);
   };
   // Infinities and NaN in V rows that a row does not see must not reach it (0 * inf):
   // in tiles with hidden keys they are stored as zeros and marked, and the rows
@@ -253,14 +244,11 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = vv[j];
     }
     if constexpr (Q8 && PAGE16) {
-      if (tid == 0) {
-        *reinterpret_cast<f32x4*>(scale_lds[st][0]) = f32x4{ksc[0], ksc[1], ksc[2], ksc[3]};
-        *reinterpret_cast<f32x4*>(scale_lds[st][1]) = f32x4{vsc[0], vsc[1], vsc[2], vsc[3]};
-      }
+      if (tid < 8) scale_lds[st][tid >> 2][tid & 3] = tile_scales;
     } else if constexpr (Q8) {
       if ((tid & 3) == 0) {
-        scale_lds[st][0][tid >> 2] = ksc[0];
-        scale_lds[st][1][tid >> 2] = vsc[0];
+        scale_lds[st][0][tid >> 2] = ksc;
+        scale_lds[st][1][tid >> 2] = vsc;
       }
     }
   };
@@ -454,22 +442,42 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int c0 = split * k.per, c1 = min(k.chunks, c0 + k.per);
   if (c0 < c1) {
     if (tid < 2) strange_lds[tid] = 0;
+    // Ahead of the tile that is computed: one in LDS, one in registers, the scales
+    // of the one behind them, and the page ids of the next.
+    auto at = [&](int c) { return min(c, c1 - 1); };
+    int id1 = 0, id2 = 0, id3 = 0;
+    float sc1 = 0.f, sc2 = 0.f;
     if constexpr (PAGE16) {
-      int lo, hi;
-      bounds(c0, lo, hi);
-      pages.begin(slot_of(min(max(key_of(c0), lo), hi)));
+      const int id0 = read_id(c0);
+      id1 = read_id(at(c0 + 1));
+      id2 = read_id(at(c0 + 2));
+      id3 = read_id(at(c0 + 3));
+      const float sc0 = pages.read_scale(id0);
+      sc1 = pages.read_scale(id1);
+      sc2 = pages.read_scale(id2);
+      load(c0, id0, sc0);
+    } else {
+      load(c0, 0, 0.f);
     }
-    load(c0);
     lds_barrier();  // (the marks are cleared)
     store(0, c0);
-    if (c0 + 1 < c1) load(c0 + 1);
+    if (c0 + 1 < c1) load(c0 + 1, id1, sc1);
     lds_barrier();
     for (int c = c0; c < c1; ++c) {
       const int st = (c - c0) & 1;
       // the next tile's registers go to the other stage, which every wave left
       // before the last barrier; then the one behind it is asked for
       if (c + 1 < c1) store(st ^ 1, c + 1);
-      if (c + 2 < c1) load(c + 2);
+      int id4 = 0;
+      float sc3 = 0.f;
+      if constexpr (PAGE16) {
+        id4 = read_id(at(c + 4));
+        sc3 = pages.read_scale(id3);
+      }
+      if (c + 2 < c1) load(c + 2, id2, sc2);
+      id2 = id3;
+      id3 = id4;
+      sc2 = sc3;
       if (computes) compute(st, c);
       lds_barrier();
     }
