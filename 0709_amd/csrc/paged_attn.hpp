@@ -261,40 +261,50 @@ __device__ __forceinline__ int slot_of(const PagedAttnArgs& a, int key) {
 }
 
 // Pages of the 16-key tiles of one step, for page sizes that are multiples of 16.
-// Lane l holds what belongs to tile l % KT: its page id, read two steps before the
-// step's rows are asked for, and its scales (K's in lanes of even l / KT, V's in the others), read one
-// step before.  The tiles' values come back by readlane, and no memory access
-// of the key loop waits for another.
+// Lane l holds what belongs to tile l % KT: its page id, read steps before the step's
+// rows are asked for; one step later the offset of the tile's first row and the
+// page's scales (K's in lanes of even l / KT, V's in the others).  The tiles' values come
+// back by readlane, and no memory access of the key loop waits for another.
 template <bool Q8, int KT>
 struct TilePages {
   const int32_t* ids;  // the request's page ids
   const float* scales;
-  int64_t scale_page;
+  int64_t scale_page, page_stride;
   int64_t last_id;  // ids are clamped to [0, last_id]
+  int page_size, ts;
 
   __device__ __forceinline__ void begin(const PagedAttnArgs& a, const Request& r, int h, int lane) {
     ids = a.p.kv_indices + r.pt;
     if constexpr (Q8)
       scales = a.p.kv_scales + int64_t(h) * a.p.scale_stride_head + ((lane / KT) & 1) * a.p.scale_stride_kv;
     scale_page = a.p.scale_stride_page;
+    page_stride = a.p.page_stride;
     last_id = a.p.num_pages - 1;
+    page_size = a.p.page_size;
+    ts = int(a.p.token_stride);
   }
-  // First key of the lane's tile of the step at kb, on a tile that holds a key of [lo, hi]
+  // First key of tile kt of the step at kb, on a tile that holds a key of [lo, hi]
   static __device__ __forceinline__ int tile_key(int kb, int kt, int lo, int hi) {
     return min(max(kb + kt * 16, lo & ~15), hi & ~15);
-  }
-  __device__ __forceinline__ int read_id(const PagedAttnArgs& a, int kb, int lo, int hi, int lane) const {
-    return ids[slot_of(a, tile_key(kb, lane & (KT - 1), lo, hi))];
   }
   __device__ __forceinline__ int64_t valid(int id) const {
     const int64_t x = id;
     return x < 0 ? 0 : (x > last_id ? last_id : x);
   }
+  // Of the lane's tile (first key `tile`):
+  __device__ __forceinline__ int read_id(const PagedAttnArgs& a, int tile) const { return ids[slot_of(a, tile)]; }
+  __device__ __forceinline__ int64_t row_offset(const PagedAttnArgs& a, int id, int tile) const {
+    return valid(id) * page_stride + int64_t((tile - slot_of(a, tile) * page_size) * ts);
+  }
   __device__ __forceinline__ float read_scale(int id) const {
     if constexpr (Q8) return scales[valid(id) * scale_page];
     else return 0.f;
   }
-  static __device__ __forceinline__ int tile_id(int v, int kt) { return __builtin_amdgcn_readlane(v, kt); }
+  static __device__ __forceinline__ int64_t tile_row(int64_t v, int kt) {
+    const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(v), kt);
+    const uint32_t hi = __builtin_amdgcn_readlane(uint32_t(uint64_t(v) >> 32), kt);
+    return int64_t((uint64_t(hi) << 32) | lo);
+  }
   static __device__ __forceinline__ float tile_scale(float v, int kv, int kt) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), kv * KT + kt));
   }

@@ -36,8 +36,8 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t* out) {
 
 // KIND: what the cache holds.  D: head_dim.  PAGE16: page_size is a multiple of 16,
 // so a 16-key tile lies in one page and its id and scales are wave-uniform;
-// other page sizes look every key up.
-template <int KIND, int D, bool PAGE16>
+// other page sizes look every key up.  SCORED: scores may be capped or biased.
+template <int KIND, int D, bool PAGE16, bool SCORED>
 __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnArgs a) {
   typedef Cache<KIND> C;
   typedef typename C::frag frag;
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
       qscale *= q_to_f16<KS>(f, qf);
     }
   }
-  const float slope = p.alibi_slopes ? p.alibi_slopes[head] * kPaLog2e : 0.f;
+  const float slope = SCORED && p.alibi_slopes ? p.alibi_slopes[head] * kPaLog2e : 0.f;
   float m_run = -INFINITY, l_run = 0.f;
   f32x4 o[DL];
 #pragma unroll
@@ -131,25 +131,27 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
     float ks[NS], vs[NS];
   };
   // first key of step s
-  auto key_of = [&](int s) {
+  auto key_of = [&](int s) __attribute__((always_inline)) {
     const int c = s / SUB;
     return (c < k.ca ? c : c - k.ca + k.cb) * kChunk + (s % SUB) * CK;
   };
-  auto bounds = [&](int s, int& lo, int& hi) {
+  auto bounds = [&](int s, int& lo, int& hi) __attribute__((always_inline)) {
     const bool first = s < k.ca * SUB;
     lo = first ? 0 : k.lo;
     hi = (first ? k.prefix : k.hi) - 1;
   };
-  auto read_id = [&](int s) {
+  typedef TilePages<Q8, KT> Tiles;
+  // first key of the lane's tile of step s
+  auto lane_tile = [&](int s) __attribute__((always_inline)) {
     int lo, hi;
     bounds(s, lo, hi);
-    return pages.read_id(a, key_of(s), lo, hi, lane);
+    return Tiles::tile_key(key_of(s), lane & (KT - 1), lo, hi);
   };
   // lane offsets of a tile's rows
   const uint32_t k_lane = uint32_t(r16 * ts + g * 16), v_lane = uint32_t(4 * g * ts + r16 * VB);
   // Keys outside [lo, hi) of the step's part repeat its nearest key, so that
   // every load falls on a row that is there.
-  auto load = [&](Raw& x, int s, int id, float scale) {
+  auto load = [&](Raw& x, int s, int64_t rows_at, float scale) __attribute__((always_inline)) {
     const int kb = key_of(s);
     int lo, hi;
     bounds(s, lo, hi);
@@ -157,17 +159,15 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
       const bool whole = kb >= lo && kb + CK <= hi + 1;
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const int tile = TilePages<Q8, KT>::tile_key(kb, kt, lo, hi);
-        const int64_t at = pages.valid(TilePages<Q8, KT>::tile_id(id, kt)) * p.page_stride;
         // the tile's first row; then lane offsets from it
-        const int64_t row0 = at + int64_t(tile - slot_of(a, tile) * page_size) * ts;
+        const int64_t row0 = Tiles::tile_row(rows_at, kt);
         const char* kp = kbase + row0;
         const char* vp = vbase + row0;
         uint32_t ko = k_lane, vo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) vo[i] = v_lane + uint32_t(i * ts);
         if (!whole) {
-          const int t0 = kb + kt * 16;
+          const int t0 = kb + kt * 16, tile = Tiles::tile_key(kb, kt, lo, hi);
           ko = uint32_t((min(max(t0 + r16, lo), hi) - tile) * ts + g * 16);
 #pragma unroll
           for (int i = 0; i < 4; ++i) vo[i] = uint32_t((min(max(t0 + 4 * g + i, lo), hi) - tile) * ts + r16 * VB);
@@ -177,12 +177,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
 #pragma unroll
         for (int i = 0; i < 4; ++i) load_words<VB>(vp + vo[i], x.v[kt][i]);
         if constexpr (Q8) {
-          x.ks[kt] = TilePages<Q8, KT>::tile_scale(scale, 0, kt);
-          x.vs[kt] = TilePages<Q8, KT>::tile_scale(scale, 1, kt);
+          x.ks[kt] = Tiles::tile_scale(scale, 0, kt);
+          x.vs[kt] = Tiles::tile_scale(scale, 1, kt);
         }
       }
     } else {
-      auto page_of = [&](int slot) { return pages.valid(pages.ids[slot]); };
+      auto page_of = [&](int slot) __attribute__((always_inline)) { return pages.valid(pages.ids[slot]); };
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
         const int t0 = kb + kt * 16;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
   // Largest V scale so far: O holds sums of p * v * (scale / vref).
   float vref = 1.17549435e-38f, vinv = 8.5070592e37f;
 
-  auto compute = [&](const Raw& x, int s) {
+  auto compute = [&](const Raw& x, int s) __attribute__((always_inline)) {
     const int kb = key_of(s);
     f32x4 acc[KT];
 #pragma unroll
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
 #pragma unroll
     for (int i = 0; i < KT * 4; ++i)
       sc[i] = acc[i >> 2][i & 3] * (Q8 ? qscale * x.ks[PAGE16 ? i >> 2 : i] : qscale);
-    if (p.soft_cap > 0.f) {
+    if (SCORED && p.soft_cap > 0.f) {
       // cap * tanh(y / cap) = cap * (1 - 2 / (1 + e^(2 y / cap))), to powers of two
 #pragma unroll
       for (int i = 0; i < KT * 4; ++i) {
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
       }
     }
     const int key0 = kb + 4 * g;
-    if (p.alibi_slopes != nullptr) {
+    if (SCORED && p.alibi_slopes != nullptr) {
 #pragma unroll
       for (int i = 0; i < KT * 4; ++i)
         sc[i] = __builtin_fmaf(-slope, fabsf(float(qpos - key0 - ((i >> 2) * 16 + (i & 3)))), sc[i]);
@@ -308,30 +308,35 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_decode_kernel(PagedAttnAr
     // The next step's rows, the scales of the one behind it and the page ids of the
     // third are in flight while a step is computed; past the last step it is asked
     // for again rather than branched around, so the waits stay exact.
-    auto at = [&](int s) { return min(s, s1 - 1); };
-    int id0 = 0, id1 = 0, id2 = 0;
+    auto at = [&](int s) __attribute__((always_inline)) { return min(s, s1 - 1); };
+    int64_t row0 = 0, row1 = 0;
+    int id2 = 0;
     float sc0 = 0.f, sc1 = 0.f;
     if constexpr (PAGE16) {
-      id0 = read_id(s0);
-      id1 = read_id(at(s0 + 1));
-      id2 = read_id(at(s0 + 2));
+      const int t0 = lane_tile(s0), t1 = lane_tile(at(s0 + 1));
+      const int id0 = pages.read_id(a, t0), id1 = pages.read_id(a, t1);
+      id2 = pages.read_id(a, lane_tile(at(s0 + 2)));
       sc0 = pages.read_scale(id0);
+      row0 = pages.row_offset(a, id0, t0);
       sc1 = pages.read_scale(id1);
+      row1 = pages.row_offset(a, id1, t1);
     }
     Raw x, y;
-    load(x, s0, id0, sc0);
+    load(x, s0, row0, sc0);
     int s = s0;
-    auto step = [&](Raw& cur, Raw& next) {
+    auto step = [&](Raw& cur, Raw& next) __attribute__((always_inline)) {
       int id3 = 0;
+      int64_t row2 = 0;
       float sc2 = 0.f;
       if constexpr (PAGE16) {
-        id3 = read_id(at(s + 3));
+        id3 = pages.read_id(a, lane_tile(at(s + 3)));
         sc2 = pages.read_scale(id2);
+        row2 = pages.row_offset(a, id2, lane_tile(at(s + 2)));
       }
-      load(next, at(s + 1), id1, sc1);
+      load(next, at(s + 1), row1, sc1);
       compute(cur, s);
-      id1 = id2;
       id2 = id3;
+      row1 = row2;
       sc1 = sc2;
       return ++s < s1;
     };

@@ -7,20 +7,30 @@
 namespace atlas {
 namespace {
 
-template <int KIND, int D, bool PAGE16>
-int launch_paged_attn(const PagedAttnArgs& a, hipStream_t stream) {
+template <int KIND, int D, bool PAGE16, bool SCORED>
+void launch_paged_kernel(const PagedAttnArgs& a, hipStream_t stream) {
   const atlas_paged_attn_t& p = a.p;
   const int64_t units = int64_t(p.batch) * p.num_kv_heads * p.num_splits;
   if (p.single_token) {
     const dim3 grid(static_cast<unsigned>(units * p.row_blocks));
-    hipLaunchKernelGGL((paged_decode_kernel<KIND, D, PAGE16>), grid, dim3(kPaThreads), 0, stream, a);
+    hipLaunchKernelGGL((paged_decode_kernel<KIND, D, PAGE16, SCORED>), grid, dim3(kPaThreads), 0, stream, a);
   } else {
     const dim3 grid(static_cast<unsigned>(p.row_blocks == 1 ? units : (units + 7) / 8 * 8 * p.row_blocks));
     if (p.block_rows <= 64)
-      hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 1, PAGE16>), grid, dim3(kPaThreads), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 1, PAGE16, SCORED>), grid, dim3(kPaThreads), 0, stream, a);
     else
-      hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 2, PAGE16>), grid, dim3(kPaThreads), 0, stream, a);
+      hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 2, PAGE16, SCORED>), grid, dim3(kPaThreads), 0, stream, a);
   }
+}
+
+template <int KIND, int D>
+int launch_paged_attn(const PagedAttnArgs& a, hipStream_t stream) {
+  const atlas_paged_attn_t& p = a.p;
+  const bool scored = p.soft_cap > 0.f || p.alibi_slopes != nullptr || p.sm_scale < 0.f;
+  // (page sizes that are no multiple of 16 are bound by looking keys up; they take the general scores)
+  if (p.page_size % 16 != 0) launch_paged_kernel<KIND, D, false, true>(a, stream);
+  else if (scored) launch_paged_kernel<KIND, D, true, true>(a, stream);
+  else launch_paged_kernel<KIND, D, true, false>(a, stream);
   int rc = launch_status("paged attention kernel");
   if (rc || p.num_splits == 1) return rc;
   const dim3 mgrid(static_cast<unsigned>(p.batch * p.num_kv_heads * p.row_blocks), p.block_rows / 4);
@@ -30,10 +40,7 @@ int launch_paged_attn(const PagedAttnArgs& a, hipStream_t stream) {
 
 template <int KIND>
 int launch_paged_attn_kind(const PagedAttnArgs& a, hipStream_t stream) {
-  const bool page16 = a.p.page_size % 16 == 0;
-  if (a.p.head_dim == 128)
-    return page16 ? launch_paged_attn<KIND, 128, true>(a, stream) : launch_paged_attn<KIND, 128, false>(a, stream);
-  return page16 ? launch_paged_attn<KIND, 64, true>(a, stream) : launch_paged_attn<KIND, 64, false>(a, stream);
+  return a.p.head_dim == 128 ? launch_paged_attn<KIND, 128>(a, stream) : launch_paged_attn<KIND, 64>(a, stream);
 }
 
 }  // namespace

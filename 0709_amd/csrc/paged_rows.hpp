@@ -34,7 +34,11 @@ __device__ __forceinline__ uint32_t below4(int key0, int end) {
   return (1u << min(max(end - key0, 0), 4)) - 1u;
 }
 
-template <int KIND, int D, int RT, bool PAGE16>
+// KIND: what the cache holds.  D: head_dim.  RT: row tiles of a wave.  PAGE16: page_size
+// is a multiple of 16, so a 16-key tile lies in one page and its id and scales are
+// wave-uniform; other page sizes look every key up.  SCORED: scores may be capped or
+// biased, or their factor negative.
+template <int KIND, int D, int RT, bool PAGE16, bool SCORED>
 __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs a) {
   typedef Cache<KIND> C;
   typedef typename C::frag frag;
@@ -121,7 +125,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     }
     m_run[rt] = -INFINITY;
     l_run[rt] = 0.f;
-    slope[rt] = p.alibi_slopes ? p.alibi_slopes[head] * kPaLog2e : 0.f;
+    slope[rt] = SCORED && p.alibi_slopes ? p.alibi_slopes[head] * kPaLog2e : 0.f;
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -134,15 +138,17 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   TilePages<Q8, 4> pages;
   pages.begin(a, r, h, lane);
 
-  auto key_of = [&](int c) { return (c < k.ca ? c : c - k.ca + k.cb) * TK; };
-  auto bounds = [&](int c, int& lo, int& hi) {
+  auto key_of = [&](int c) __attribute__((always_inline)) { return (c < k.ca ? c : c - k.ca + k.cb) * TK; };
+  auto bounds = [&](int c, int& lo, int& hi) __attribute__((always_inline)) {
     lo = c < k.ca ? 0 : k.lo;
     hi = (c < k.ca ? k.prefix : k.hi) - 1;
   };
-  auto read_id = [&](int c) {
+  typedef TilePages<Q8, 4> Tiles;
+  // first key of the lane's 16-key tile of tile c
+  auto lane_tile = [&](int c) __attribute__((always_inline)) {
     int lo, hi;
     bounds(c, lo, hi);
-    return pages.read_id(a, key_of(c), lo, hi, lane);
+    return Tiles::tile_key(key_of(c), lane & 3, lo, hi);
   };
   // Piece j of a thread: row (j * 256 + tid) / GG of the tile, piece tid % GG of it.
   const int piece = tid % GG, prow0 = tid / GG;
@@ -151,7 +157,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   float tile_scales = 0.f;       // scales of the tile in kraw / vraw, as read
   float ksc = 0.f, vsc = 0.f;    // other page sizes: those of key tid / 4
   // Keys outside [lo, hi) of the tile's part repeat its nearest key.
-  auto load = [&](int c, int id, float scale) {
+  auto load = [&](int c, int64_t rows_at, float scale) __attribute__((always_inline)) {
     const int kb = key_of(c);
     int lo, hi;
     bounds(c, lo, hi);
@@ -161,9 +167,8 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       if constexpr (PAGE16) {
         // (a wave's rows of one piece lie in one 16-key tile)
         const int kt = (j * RSTEP + wave * (64 / GG)) >> 4;
-        const int tile = TilePages<Q8, 4>::tile_key(kb, kt, lo, hi);
-        const int64_t row0 = pages.valid(__builtin_amdgcn_readlane(id, kt)) * p.page_stride +
-                             int64_t(tile - slot_of(a, tile) * page_size) * ts;
+        const int64_t row0 = Tiles::tile_row(rows_at, kt);
+        const int tile = Tiles::tile_key(kb, kt, lo, hi);
         const uint32_t off = uint32_t((key - tile) * ts + piece * 16);
         kraw[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
         vraw[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);
@@ -185,28 +190,32 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   // Does some key of tile c hide from some row?
   const int plain_hi = p.mask_mode == 2 ? shift + k.n0 + 1 : (p.mask_mode == 1 ? min(r.kv_len, col0) : r.kv_len);
   const int plain_lo = p.mask_mode == 2 && p.window_left >= 0 ? shift + k.n1 - p.window_left : 0;
-  auto masked_tile = [&](int kb) {
+  auto masked_tile = [&](int kb) __attribute__((always_inline)) {
     return ((kb + TK > plain_hi) | (kb < plain_lo)) & (kb + TK > k.prefix);
   };
   // Infinities and NaN in V rows that a row does not see must not reach it (0 * inf):
   // in tiles with hidden keys they are stored as zeros and marked, and the rows
   // that see them get them from the marks.
-  auto take_out = [&](frag v, int st, int row, int gr) {
-    constexpr uint32_t kExp = C::kBf16 ? 0x7f80u : 0x7c00u;
+  // Both halves of a word at a time: the exponent's carry marks what is not finite, the
+  // mantissa's carry NaN.
+  auto take_out = [&](frag v, int st, int row, int gr, uint32_t& odd) __attribute__((always_inline)) {
+    constexpr uint32_t kExp = C::kBf16 ? 0x7f807f80u : 0x7c007c00u, kLow = C::kBf16 ? 0x00800080u : 0x04000400u;
+    constexpr uint32_t kMan = C::kBf16 ? 0x007f007fu : 0x03ff03ffu, kTop = 0x80008000u;
     uint32_t up = 0, dn = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t x = (v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-      const uint32_t bad = (x & kExp) == kExp ? 1u : 0u, nan = (x & 0x7fffu) > kExp ? 1u : 0u, neg = x >> 15;
-      up |= (bad & (nan | (neg ^ 1u))) << i;
-      dn |= (bad & (nan | neg)) << i;
-      if (bad) v[i >> 1] &= i & 1 ? 0xffffu : 0xffff0000u;
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t x = v[w], bad = ((x & kExp) + kLow) & kTop, nan = (x & kMan) + 0x7fff7fffu;
+      const uint32_t u = bad & (nan | ~x), d = bad & (nan | x);
+      up |= ((u >> 15 & 1u) | (u >> 30 & 2u)) << (2 * w);
+      dn |= ((d >> 15 & 1u) | (d >> 30 & 2u)) << (2 * w);
+      v[w] = x & ~((bad << 1) - (bad >> 15));
+      odd |= bad;
     }
     up_lds[st][row * (D / 8) + gr] = uint8_t(up);
     dn_lds[st][row * (D / 8) + gr] = uint8_t(dn);
     return v;
   };
-  auto store = [&](int st, int c) {
+  auto store = [&](int st, int c) __attribute__((always_inline)) {
     char* kd = lds[st];
     char* vd = lds[st] + HALF;
     frag vv[Q8 ? 2 * NL : NL];
@@ -226,17 +235,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       }
     }
     if (KIND != kCacheInt8 && masked_tile(key_of(c))) {
-      constexpr uint32_t kExp = C::kBf16 ? 0x7f807f80u : 0x7c007c00u, kLow = C::kBf16 ? 0x00800080u : 0x04000400u;
-      uint32_t odd = 0;  // (an exponent of all ones carries into the sign's place)
+      // (the marks of a tile are whole: every thread writes its part, whether it has some or not)
+      uint32_t odd = 0;
 #pragma unroll
       for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) odd |= (vv[j][w] & kExp) + kLow;
-      // (the marks of a tile are whole: every wave writes its part, whether it has some or not)
-#pragma unroll
-      for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j)
-        vv[j] = take_out(vv[j], st, (Q8 ? j >> 1 : j) * RSTEP + prow0, Q8 ? 2 * piece + (j & 1) : piece);
-      if (odd & 0x80008000u) strange_lds[st] = c + 1;
+        vv[j] = take_out(vv[j], st, (Q8 ? j >> 1 : j) * RSTEP + prow0, Q8 ? 2 * piece + (j & 1) : piece, odd);
+      if (odd) strange_lds[st] = c + 1;
     }
 #pragma unroll
     for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j) {
@@ -261,11 +265,11 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int vkey = 4 * g + e4;
 
   // One tile for this wave's row tiles, 32 keys at a time.
-  auto compute = [&](int st, int c) {
+  auto compute = [&](auto masked_tag, int st, int c) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(masked_tag)::value;
     const int kb = key_of(c);
     const char* kd = lds[st];
     const char* vd = lds[st] + HALF;
-    const bool masked = masked_tile(kb);
     const bool strange = masked && KIND != kCacheInt8 && strange_lds[st] == c + 1;
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
@@ -323,10 +327,13 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
 #pragma unroll
         for (int i = 0; i < (PAGE16 || !Q8 ? 2 : 8); ++i)
           f[i] = !Q8 ? qscale[rt] : qscale[rt] * (PAGE16 ? ksk[i][0] : ksk[i >> 2][i & 3]);
-        const bool plain = p.soft_cap == 0.f && p.alibi_slopes == nullptr && !masked && p.sm_scale >= 0.f;
-        if (!plain) {
+        if constexpr (SCORED || masked) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= f[PAGE16 || !Q8 ? i >> 2 : i];
+#pragma unroll
+          for (int i = 0; i < (PAGE16 || !Q8 ? 2 : 8); ++i) f[i] = 1.f;
+        }
+        if constexpr (SCORED) {
           if (p.soft_cap > 0.f) {
             // cap * tanh(y / cap) = cap * (1 - 2 / (1 + e^(2 y / cap))), to powers of two
 #pragma unroll
@@ -337,14 +344,18 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
           }
           if (p.alibi_slopes != nullptr) {
             const float away = float(qpos - key0);
+            if (kb + TK <= shift + k.n0 + 1) {  // no key of the tile stands behind a query
+              const float b0 = -slope[rt] * away;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              x[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), x[i]);
+              for (int i = 0; i < 8; ++i) x[i] += __builtin_fmaf(slope[rt], float((i >> 2) * 16 + (i & 3)), b0);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                x[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), x[i]);
+            }
           }
-#pragma unroll
-          for (int i = 0; i < (PAGE16 || !Q8 ? 2 : 8); ++i) f[i] = 1.f;
         }
-        if (masked) {
+        if constexpr (masked) {
           uint64_t w = 0;
           int w0 = col0;
           if (p.mask_mode == 1) {
@@ -414,7 +425,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf, pf[rt], o[rt][t]);
       }
-      if (strange) {
+      if (masked && strange) {
         // Where a row sees an infinity or NaN, its sum becomes one: a product with the
         // marks is zero for the rows that do not.
         constexpr uint32_t kOne = C::kBf16 ? 0x3f80u : 0x3c00u;
@@ -444,42 +455,52 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     if (tid < 2) strange_lds[tid] = 0;
     // Ahead of the tile that is computed: one in LDS, one in registers, the scales
     // of the one behind them, and the page ids of the next.
-    auto at = [&](int c) { return min(c, c1 - 1); };
-    int id1 = 0, id2 = 0, id3 = 0;
+    auto at = [&](int c) __attribute__((always_inline)) { return min(c, c1 - 1); };
+    int64_t row1 = 0, row2 = 0;
+    int id3 = 0;
     float sc1 = 0.f, sc2 = 0.f;
     if constexpr (PAGE16) {
-      const int id0 = read_id(c0);
-      id1 = read_id(at(c0 + 1));
-      id2 = read_id(at(c0 + 2));
-      id3 = read_id(at(c0 + 3));
+      const int t0 = lane_tile(c0), t1 = lane_tile(at(c0 + 1)), t2 = lane_tile(at(c0 + 2));
+      const int id0 = pages.read_id(a, t0), id1 = pages.read_id(a, t1), id2 = pages.read_id(a, t2);
+      id3 = pages.read_id(a, lane_tile(at(c0 + 3)));
       const float sc0 = pages.read_scale(id0);
       sc1 = pages.read_scale(id1);
       sc2 = pages.read_scale(id2);
-      load(c0, id0, sc0);
+      row1 = pages.row_offset(a, id1, t1);
+      row2 = pages.row_offset(a, id2, t2);
+      load(c0, pages.row_offset(a, id0, t0), sc0);
     } else {
       load(c0, 0, 0.f);
     }
     lds_barrier();  // (the marks are cleared)
     store(0, c0);
-    if (c0 + 1 < c1) load(c0 + 1, id1, sc1);
+    if (c0 + 1 < c1) load(c0 + 1, row1, sc1);
     lds_barrier();
-    for (int c = c0; c < c1; ++c) {
+    auto step = [&](auto masked_tag, int c) __attribute__((always_inline)) {
       const int st = (c - c0) & 1;
       // the next tile's registers go to the other stage, which every wave left
       // before the last barrier; then the one behind it is asked for
       if (c + 1 < c1) store(st ^ 1, c + 1);
       int id4 = 0;
+      int64_t row3 = 0;
       float sc3 = 0.f;
       if constexpr (PAGE16) {
-        id4 = read_id(at(c + 4));
+        id4 = pages.read_id(a, lane_tile(at(c + 4)));
         sc3 = pages.read_scale(id3);
+        row3 = pages.row_offset(a, id3, lane_tile(at(c + 3)));
       }
-      if (c + 2 < c1) load(c + 2, id2, sc2);
-      id2 = id3;
+      if (c + 2 < c1) load(c + 2, row2, sc2);
       id3 = id4;
+      row2 = row3;
       sc2 = sc3;
-      if (computes) compute(st, c);
+      if (computes) compute(masked_tag, st, c);
       lds_barrier();
+    };
+    // Runs of tiles without hidden keys take the shorter form.
+    int c = c0;
+    while (c < c1) {
+      for (; c < c1 && masked_tile(key_of(c)); ++c) step(std::true_type{}, c);
+      for (; c < c1 && !masked_tile(key_of(c)); ++c) step(std::false_type{}, c);
     }
   }
 

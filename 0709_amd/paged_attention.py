@@ -41,7 +41,10 @@ WIDE_BLOCK_ROWS = 128
 # Requests of more packed rows than this take the wide blocks.
 MAX_NARROW_ROWS = 192
 # Workgroups to aim for when the keys are split, and the least keys of a split.
+# Decode splits are never longer than MAX_DECODE_SPLIT keys where the batch is
+# large: short splits even out requests of different lengths.
 DECODE_WORKGROUPS = 1024
+MAX_DECODE_SPLIT = 1024
 BLOCK_WORKGROUPS = 512
 MIN_SPLIT_KEYS = 256
 MAX_SPLITS = 256
@@ -69,8 +72,11 @@ def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_l
         blocks = -(-rows // (BLOCK_ROWS if rows <= MAX_NARROW_ROWS else WIDE_BLOCK_ROWS))
         block_rows, target = 16 * -(-rows // (16 * blocks)), BLOCK_WORKGROUPS
     items = batch * kv_heads * blocks
-    most = min(MAX_SPLITS, max(1, -(-max_kv_len // MIN_SPLIT_KEYS)))
-    splits = max(1, min(most, target // items))
+    most = max(1, -(-max_kv_len // MIN_SPLIT_KEYS))
+    splits = min(most, target // items)
+    if single:
+        splits = max(splits, -(-max_kv_len // MAX_DECODE_SPLIT)) if max_kv_len > MAX_DECODE_SPLIT else 1
+    splits = max(1, min(MAX_SPLITS, splits))
     keys = max(64, -(-max_kv_len // splits))
     keys = -(-keys // 64) * 64
     return single, block_rows, blocks, max(1, -(-max_kv_len // keys)), keys
