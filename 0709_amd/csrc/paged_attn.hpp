@@ -3,8 +3,8 @@
 // capped, biased by distance, windowed or masked by a draft tree's words.
 // This file: what the two kernels share, and the join of key splits.
 //
-//   paged_decode.hpp  one query token per request, up to 16 packed rows;
-//   paged_rows.hpp    everything else.
+//   paged_stream.hpp  few packed rows: one query token per request, or short blocks;
+//   paged_rows.hpp    many rows.
 //
 // Rows are packed: row = query token * group + head of the group, for one KV head.
 //
@@ -132,6 +132,34 @@ __device__ __forceinline__ float groups_sum(float v) {
   v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
   r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Bits of the four keys key0 .. key0 + 3 below `end`.
+__device__ __forceinline__ uint32_t below4(int key0, int end) {
+  return (1u << min(max(end - key0, 0), 4)) - 1u;
+}
+// Those that a word of tree columns shows, the first of them `off` columns behind the
+// word's start (columns before it are the prefix, those past its end are hidden).
+__device__ __forceinline__ uint32_t tree4(uint64_t w, int off) {
+  const int pre = min(max(-off, 0), 4);
+  const uint32_t up = off >= 0 && off < 64 ? uint32_t(w >> (off & 63)) : 0u;
+  const uint32_t down = uint32_t(w << pre) | ((1u << pre) - 1u);
+  return off >= 0 ? up : down;
+}
+
+// Two 16-bit values at a time: the exponent's carry (bits 15 and 31) marks what is
+// not finite, the mantissa's carry NaN.
+template <bool BF16>
+__device__ __forceinline__ uint32_t not_finite2(uint32_t x) {
+  return ((x & (BF16 ? 0x7f807f80u : 0x7c007c00u)) + (BF16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+// The values with zeros for what is not finite; u marks +inf and NaN, d -inf and NaN.
+template <bool BF16>
+__device__ __forceinline__ uint32_t take_out2(uint32_t x, uint32_t& u, uint32_t& d) {
+  const uint32_t bad = not_finite2<BF16>(x), nan = (x & (BF16 ? 0x007f007fu : 0x03ff03ffu)) + 0x7fff7fffu;
+  u = bad & (nan | ~x);
+  d = bad & (nan | x);
+  return x & ~((bad << 1) - (bad >> 15));
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {

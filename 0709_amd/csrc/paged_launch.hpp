@@ -1,8 +1,8 @@
 // Launches of the paged attention kernels over one kind of cache.
 #pragma once
 
-#include "paged_decode.hpp"
 #include "paged_rows.hpp"
+#include "paged_stream.hpp"
 
 namespace atlas {
 namespace {
@@ -11,16 +11,15 @@ template <int KIND, int D, bool PAGE16, bool SCORED>
 void launch_paged_kernel(const PagedAttnArgs& a, hipStream_t stream) {
   const atlas_paged_attn_t& p = a.p;
   const int64_t units = int64_t(p.batch) * p.num_kv_heads * p.num_splits;
-  if (p.single_token) {
-    const dim3 grid(static_cast<unsigned>(units * p.row_blocks));
-    hipLaunchKernelGGL((paged_decode_kernel<KIND, D, PAGE16, SCORED>), grid, dim3(kPaThreads), 0, stream, a);
-  } else {
-    const dim3 grid(static_cast<unsigned>(p.row_blocks == 1 ? units : (units + 7) / 8 * 8 * p.row_blocks));
-    if (p.block_rows <= 64)
-      hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 1, PAGE16, SCORED>), grid, dim3(kPaThreads), 0, stream, a);
-    else
-      hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 2, PAGE16, SCORED>), grid, dim3(kPaThreads), 0, stream, a);
-  }
+  const dim3 grid(static_cast<unsigned>(p.row_blocks == 1 ? units : (units + 7) / 8 * 8 * p.row_blocks)), block(kPaThreads);
+  if (p.single_token)
+    hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 1, PAGE16, SCORED, false>), grid, block, 0, stream, a);
+  else if (p.block_rows <= 16)
+    hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 1, PAGE16, SCORED, true>), grid, block, 0, stream, a);
+  else if (PAGE16 && p.block_rows <= 64)
+    hipLaunchKernelGGL((paged_rows_kernel<KIND, D, PAGE16 ? 1 : 2, PAGE16, SCORED>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 2, PAGE16, SCORED>), grid, block, 0, stream, a);
 }
 
 template <int KIND, int D>

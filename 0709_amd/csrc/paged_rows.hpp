@@ -1,5 +1,4 @@
-// Paged attention for several query tokens per request: prompts' chunks, draft
-// trees, short batches.
+// Paged attention for many packed rows: prompts' chunks and wide draft trees.
 //
 // A workgroup of four waves takes up to 64 * RT packed rows of one KV head and one
 // split of the request's keys.  Tiles of 64 keys go from HBM through registers into
@@ -29,11 +28,6 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Bits of the four keys key0 .. key0 + 3 below `end`.
-__device__ __forceinline__ uint32_t below4(int key0, int end) {
-  return (1u << min(max(end - key0, 0), 4)) - 1u;
-}
-
 // KIND: what the cache holds.  D: head_dim.  RT: row tiles of a wave.  PAGE16: page_size
 // is a multiple of 16, so a 16-key tile lies in one page and its id and scales are
 // wave-uniform; other page sizes look every key up.  SCORED: scores may be capped or
@@ -51,6 +45,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   constexpr int HALF = TK * RB;            // K's or V's half of a stage
   constexpr int GG = D * C::kBytes / 16;   // 16-byte pieces of a row in the cache
   constexpr int NL = TK * GG / kPaThreads; // pieces a thread carries, of K and of V
+  constexpr int SETS = Q8 && RT == 1 ? 2 : 1;  // tiles in flight in registers
   constexpr int KSW = GR - 1;              // granule swaps: K by key, V by key pairs
   constexpr int VSW = GR / 2 - 1;
   const atlas_paged_attn_t& p = a.p;
@@ -153,11 +148,13 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   // Piece j of a thread: row (j * 256 + tid) / GG of the tile, piece tid % GG of it.
   const int piece = tid % GG, prow0 = tid / GG;
   constexpr int RSTEP = kPaThreads / GG;  // rows between a thread's pieces
-  w4 kraw[NL], vraw[NL];
-  float tile_scales = 0.f;       // scales of the tile in kraw / vraw, as read
-  float ksc = 0.f, vsc = 0.f;    // other page sizes: those of key tid / 4
+  struct Raw {
+    w4 k[NL], v[NL];
+    float scales;    // of the 16-key tiles, as read
+    float ks, vs;    // other page sizes: those of key tid / 4
+  };
   // Keys outside [lo, hi) of the tile's part repeat its nearest key.
-  auto load = [&](int c, int64_t rows_at, float scale) __attribute__((always_inline)) {
+  auto load = [&](Raw& x, int c, int64_t rows_at, float scale) __attribute__((always_inline)) {
     const int kb = key_of(c);
     int lo, hi;
     bounds(c, lo, hi);
@@ -170,21 +167,21 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         const int64_t row0 = Tiles::tile_row(rows_at, kt);
         const int tile = Tiles::tile_key(kb, kt, lo, hi);
         const uint32_t off = uint32_t((key - tile) * ts + piece * 16);
-        kraw[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
-        vraw[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);
+        x.k[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
+        x.v[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);
       } else {
         const int slot = slot_of(a, key);
         const int64_t at = pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts + piece * 16;
-        kraw[j] = *reinterpret_cast<const w4*>(kbase + at);
-        vraw[j] = *reinterpret_cast<const w4*>(vbase + at);
+        x.k[j] = *reinterpret_cast<const w4*>(kbase + at);
+        x.v[j] = *reinterpret_cast<const w4*>(vbase + at);
       }
     }
-    tile_scales = scale;
+    x.scales = scale;
     if constexpr (Q8 && !PAGE16) {
       const int slot = slot_of(a, min(max(kb + (tid >> 2), lo), hi));
       const float* s = p.kv_scales + int64_t(h) * p.scale_stride_head + pages.valid(pages.ids[slot]) * p.scale_stride_page;
-      ksc = s[0];
-      vsc = s[p.scale_stride_kv];
+      x.ks = s[0];
+      x.vs = s[p.scale_stride_kv];
     }
   };
   // Does some key of tile c hide from some row?
@@ -196,26 +193,21 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   // Infinities and NaN in V rows that a row does not see must not reach it (0 * inf):
   // in tiles with hidden keys they are stored as zeros and marked, and the rows
   // that see them get them from the marks.
-  // Both halves of a word at a time: the exponent's carry marks what is not finite, the
-  // mantissa's carry NaN.
   auto take_out = [&](frag v, int st, int row, int gr, uint32_t& odd) __attribute__((always_inline)) {
-    constexpr uint32_t kExp = C::kBf16 ? 0x7f807f80u : 0x7c007c00u, kLow = C::kBf16 ? 0x00800080u : 0x04000400u;
-    constexpr uint32_t kMan = C::kBf16 ? 0x007f007fu : 0x03ff03ffu, kTop = 0x80008000u;
     uint32_t up = 0, dn = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const uint32_t x = v[w], bad = ((x & kExp) + kLow) & kTop, nan = (x & kMan) + 0x7fff7fffu;
-      const uint32_t u = bad & (nan | ~x), d = bad & (nan | x);
+      uint32_t u, d;
+      v[w] = take_out2<C::kBf16>(v[w], u, d);
       up |= ((u >> 15 & 1u) | (u >> 30 & 2u)) << (2 * w);
       dn |= ((d >> 15 & 1u) | (d >> 30 & 2u)) << (2 * w);
-      v[w] = x & ~((bad << 1) - (bad >> 15));
-      odd |= bad;
+      odd |= u | d;
     }
     up_lds[st][row * (D / 8) + gr] = uint8_t(up);
     dn_lds[st][row * (D / 8) + gr] = uint8_t(dn);
     return v;
   };
-  auto store = [&](int st, int c) __attribute__((always_inline)) {
+  auto store = [&](const Raw& x, int st, int c) __attribute__((always_inline)) {
     char* kd = lds[st];
     char* vd = lds[st] + HALF;
     frag vv[Q8 ? 2 * NL : NL];
@@ -223,14 +215,14 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     for (int j = 0; j < NL; ++j) {
       const int row = j * RSTEP + prow0;
       if constexpr (!Q8) {
-        *reinterpret_cast<w4*>(kd + row * RB + ((piece ^ (row & KSW)) << 4)) = kraw[j];
-        vv[j] = vraw[j];
+        *reinterpret_cast<w4*>(kd + row * RB + ((piece ^ (row & KSW)) << 4)) = x.k[j];
+        vv[j] = x.v[j];
       } else {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           *reinterpret_cast<frag*>(kd + row * RB + (((2 * piece + e) ^ (row & KSW)) << 4)) =
-              C::keys8(kraw[j][2 * e], kraw[j][2 * e + 1]);
-          vv[2 * j + e] = C::keys8(vraw[j][2 * e], vraw[j][2 * e + 1]);
+              C::keys8(x.k[j][2 * e], x.k[j][2 * e + 1]);
+          vv[2 * j + e] = C::keys8(x.v[j][2 * e], x.v[j][2 * e + 1]);
         }
       }
     }
@@ -248,11 +240,11 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = vv[j];
     }
     if constexpr (Q8 && PAGE16) {
-      if (tid < 8) scale_lds[st][tid >> 2][tid & 3] = tile_scales;
+      if (tid < 8) scale_lds[st][tid >> 2][tid & 3] = x.scales;
     } else if constexpr (Q8) {
       if ((tid & 3) == 0) {
-        scale_lds[st][0][tid >> 2] = ksc;
-        scale_lds[st][1][tid >> 2] = vsc;
+        scale_lds[st][0][tid >> 2] = x.ks;
+        scale_lds[st][1][tid >> 2] = x.vs;
       }
     }
   };
@@ -373,11 +365,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
             if (p.mask_mode == 2) {
               vis &= (below4(at, qpos + 1) & ~below4(at, wlo)) | below4(at, k.prefix);
             } else if (p.mask_mode == 1) {
-              const int off = at - w0;  // the lane's keys in the word; those before it are the prefix
-              const int pre = min(max(-off, 0), 4);
-              const uint32_t up = off >= 0 && off < 64 ? uint32_t(w >> (off & 63)) : 0u;
-              const uint32_t down = uint32_t(w << pre) | ((1u << pre) - 1u);
-              vis &= off >= 0 ? up : down;
+              vis &= tree4(w, at - w0);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[kt * 4 + i] = (vis >> i) & 1u ? x[kt * 4 + i] : -INFINITY;
@@ -453,54 +441,74 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int c0 = split * k.per, c1 = min(k.chunks, c0 + k.per);
   if (c0 < c1) {
     if (tid < 2) strange_lds[tid] = 0;
-    // Ahead of the tile that is computed: one in LDS, one in registers, the scales
+    // Ahead of the tile that is computed: one in LDS, SETS in registers, the scales
     // of the one behind them, and the page ids of the next.
-    auto at = [&](int c) __attribute__((always_inline)) { return min(c, c1 - 1); };
-    int64_t row1 = 0, row2 = 0;
-    int id3 = 0;
-    float sc1 = 0.f, sc2 = 0.f;
-    if constexpr (PAGE16) {
-      const int t0 = lane_tile(c0), t1 = lane_tile(at(c0 + 1)), t2 = lane_tile(at(c0 + 2));
-      const int id0 = pages.read_id(a, t0), id1 = pages.read_id(a, t1), id2 = pages.read_id(a, t2);
-      id3 = pages.read_id(a, lane_tile(at(c0 + 3)));
-      const float sc0 = pages.read_scale(id0);
-      sc1 = pages.read_scale(id1);
-      sc2 = pages.read_scale(id2);
-      row1 = pages.row_offset(a, id1, t1);
-      row2 = pages.row_offset(a, id2, t2);
-      load(c0, pages.row_offset(a, id0, t0), sc0);
-    } else {
-      load(c0, 0, 0.f);
-    }
+    auto at = [&](int c) { return min(c, c1 - 1); };
+    int64_t rows_at = 0;
+    int id = 0;
+    float sc = 0.f;
+    Raw x[SETS];
+    auto first_load = [&](Raw& y, int c) __attribute__((always_inline)) {
+      int64_t rows = 0;
+      float scale = 0.f;
+      if constexpr (PAGE16) {
+        const int t = lane_tile(at(c)), i = pages.read_id(a, t);
+        rows = pages.row_offset(a, i, t);
+        scale = pages.read_scale(i);
+      }
+      load(y, at(c), rows, scale);
+    };
+    first_load(x[0], c0);
     lds_barrier();  // (the marks are cleared)
-    store(0, c0);
-    if (c0 + 1 < c1) load(c0 + 1, row1, sc1);
+    store(x[0], 0, c0);
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) first_load(x[i], c0 + 1 + i);
+    if constexpr (PAGE16) {
+      const int t = lane_tile(at(c0 + 1 + SETS)), i = pages.read_id(a, t);
+      rows_at = pages.row_offset(a, i, t);
+      sc = pages.read_scale(i);
+      id = pages.read_id(a, lane_tile(at(c0 + 2 + SETS)));
+    }
     lds_barrier();
-    auto step = [&](auto masked_tag, int c) __attribute__((always_inline)) {
+    auto step = [&](auto masked_tag, Raw& y, int c) __attribute__((always_inline)) {
       const int st = (c - c0) & 1;
       // the next tile's registers go to the other stage, which every wave left
-      // before the last barrier; then the one behind it is asked for
-      if (c + 1 < c1) store(st ^ 1, c + 1);
-      int id4 = 0;
-      int64_t row3 = 0;
-      float sc3 = 0.f;
+      // before the last barrier; then the one SETS behind it is asked for
+      if (c + 1 < c1) store(y, st ^ 1, c + 1);
+      int next_id = 0;
+      int64_t next_rows = 0;
+      float next_sc = 0.f;
       if constexpr (PAGE16) {
-        id4 = pages.read_id(a, lane_tile(at(c + 4)));
-        sc3 = pages.read_scale(id3);
-        row3 = pages.row_offset(a, id3, lane_tile(at(c + 3)));
+        next_id = pages.read_id(a, lane_tile(at(c + 3 + SETS)));
+        next_sc = pages.read_scale(id);
+        next_rows = pages.row_offset(a, id, lane_tile(at(c + 2 + SETS)));
       }
-      if (c + 2 < c1) load(c + 2, row2, sc2);
-      id3 = id4;
-      row2 = row3;
-      sc2 = sc3;
+      if (c + 1 + SETS < c1) load(y, c + 1 + SETS, rows_at, sc);
+      id = next_id;
+      rows_at = next_rows;
+      sc = next_sc;
       if (computes) compute(masked_tag, st, c);
       lds_barrier();
     };
-    // Runs of tiles without hidden keys take the shorter form.
+    // Runs of tiles without hidden keys take the shorter form.  (A choice at every tile
+    // would keep both forms' registers alive.)
     int c = c0;
     while (c < c1) {
-      for (; c < c1 && masked_tile(key_of(c)); ++c) step(std::true_type{}, c);
-      for (; c < c1 && !masked_tile(key_of(c)); ++c) step(std::false_type{}, c);
+      if constexpr (SETS == 1) {
+        for (; c < c1 && masked_tile(key_of(c)); ++c) step(std::true_type{}, x[0], c);
+        for (; c < c1 && !masked_tile(key_of(c)); ++c) step(std::false_type{}, x[0], c);
+      } else {
+        // (the sets alternate, so tiles come in pairs)
+        auto masked_pair = [&](int c) { return masked_tile(key_of(c)) || (c + 1 < c1 && masked_tile(key_of(c + 1))); };
+        for (; c < c1 && masked_pair(c); c += 2) {
+          step(std::true_type{}, x[0], c);
+          if (c + 1 < c1) step(std::true_type{}, x[SETS - 1], c + 1);
+        }
+        for (; c < c1 && !masked_pair(c); c += 2) {
+          step(std::false_type{}, x[0], c);
+          if (c + 1 < c1) step(std::false_type{}, x[SETS - 1], c + 1);
+        }
+      }
     }
   }
 

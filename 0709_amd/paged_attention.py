@@ -33,18 +33,17 @@ from . import _lib
 from .tree_attention import _host_lists
 
 # Most packed query rows (query token * group + head of the group) of a workgroup:
-# of the decode kernel, and of the kernel for several tokens with one and with two
-# row tiles a wave.
-DECODE_ROWS = 16
-BLOCK_ROWS = 64
-WIDE_BLOCK_ROWS = 128
+# the kernel of few rows, and that of many rows with one and with two row tiles a wave.
+STREAM_ROWS = 16
+NARROW_ROWS = 64
+WIDE_ROWS = 128
 # Requests of more packed rows than this take the wide blocks.
 MAX_NARROW_ROWS = 192
 # Workgroups to aim for when the keys are split, and the least keys of a split.
 # Decode splits are never longer than MAX_DECODE_SPLIT keys where the batch is
 # large: short splits even out requests of different lengths.
 DECODE_WORKGROUPS = 1024
-MAX_DECODE_SPLIT = 1024
+MAX_DECODE_SPLIT = 1536
 BLOCK_WORKGROUPS = 512
 MIN_SPLIT_KEYS = 256
 MAX_SPLITS = 256
@@ -55,22 +54,24 @@ CACHE_CODES = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8
 _ARGS = struct.Struct("=14Q15q15i2f4x")
 
 
-def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int,
-                 tree: bool = False) -> tuple[bool, int, int, int, int]:
+def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int, *, tree: bool = False,
+                 page_size: int = 16) -> tuple[bool, int, int, int, int]:
     """(single token?, rows of a block, row blocks, splits, keys per split) of a call.
 
-    One query token per request takes the decode kernel with blocks of 16 packed
-    rows, more take equal blocks.  Keys are split until about as many workgroups are
-    there as the device holds at once, in splits of at least MIN_SPLIT_KEYS; a
-    request shorter than ``max_kv_len`` takes fewer splits of the same size."""
+    One query token per request takes blocks of 16 packed rows, more take equal
+    blocks.  Keys are split until about as many workgroups are there as the device
+    holds at once, in splits of at least MIN_SPLIT_KEYS; a request shorter than
+    ``max_kv_len`` takes fewer splits of the same size."""
     single = max_q_len <= 1 and not tree
     rows = max(1, max_q_len * group)
-    if single:
-        block_rows, target = DECODE_ROWS, DECODE_WORKGROUPS
-        blocks = -(-rows // DECODE_ROWS)
+    if single or rows <= STREAM_ROWS:
+        most_rows, target = STREAM_ROWS, DECODE_WORKGROUPS
+    elif rows <= MAX_NARROW_ROWS and page_size % 16 == 0:
+        most_rows, target = NARROW_ROWS, BLOCK_WORKGROUPS
     else:
-        blocks = -(-rows // (BLOCK_ROWS if rows <= MAX_NARROW_ROWS else WIDE_BLOCK_ROWS))
-        block_rows, target = 16 * -(-rows // (16 * blocks)), BLOCK_WORKGROUPS
+        most_rows, target = WIDE_ROWS, BLOCK_WORKGROUPS
+    blocks = -(-rows // most_rows)
+    block_rows = 16 * -(-rows // (16 * blocks))
     items = batch * kv_heads * blocks
     most = max(1, -(-max_kv_len // MIN_SPLIT_KEYS))
     splits = min(most, target // items)
@@ -254,7 +255,8 @@ def paged_attention(
     max_q_len = min(int(max_q_len), nnz)
     # (keys that a window leaves to a row block; the visible prefix comes on top)
     reach = max_kv_len if window_left < 0 or prefix_lens is not None else min(max_kv_len, window_left + max_q_len)
-    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach), mode == _lib.MASK_TREE)
+    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach), tree=mode == _lib.MASK_TREE,
+                         page_size=page_size)
     need = workspace_bytes(batch, hkv, d, shape)
     if need:
         if workspace is None:

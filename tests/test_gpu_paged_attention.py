@@ -354,3 +354,13 @@ def test_other_score_scales(dev, cache, scale):
     check(s, call(dev, s, causal=True, sm_scale=scale), causal=True, sm_scale=scale)
     one = build(82, [1, 1], [100, 70], cache=cache)
     check(one, call(dev, one, causal=True, window_left=40, sm_scale=scale), causal=True, window_left=40, sm_scale=scale)
+
+
+def test_nan_scores_reach_their_rows(dev):
+    """A visible NaN key makes its row NaN (and no other), whichever wave or split holds it."""
+    for length, spot in ((70, 3), (70, 69), (3000, 100), (3000, 2990)):
+        s = build(91, [1, 1], [length, length], hq=8, hkv=2, layout="HND")
+        s["cache"][s["table"][spot // 16].long(), 0, 1, spot % 16, 5] = math.nan
+        out, lse = call(dev, s)
+        assert torch.isnan(out[0, 4:]).all() and torch.isnan(lse[0, 4:]).all()
+        assert torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1]).all() and torch.isfinite(lse[1]).all()
