@@ -28,6 +28,9 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+template <int N>
+using Stage = std::integral_constant<int, N>;
+
 // KIND: what the cache holds.  D: head_dim.  RT: row tiles of a wave.  PAGE16: page_size
 // is a multiple of 16, so a 16-key tile lies in one page and its id and scales are
 // wave-uniform; other page sizes look every key up.  SCORED: scores may be capped or
@@ -37,7 +40,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   typedef Cache<KIND> C;
   typedef typename C::frag frag;
   constexpr bool Q8 = C::kQuant;
-  constexpr int TK = kChunk;               // keys of a tile
+  constexpr int TK = D == 128 ? 32 : 64;  // keys of a tile
+  constexpr int SUB = kChunk / TK;         // tiles of a chunk
+  constexpr int NT = TK / 16;              // its 16-key tiles
   constexpr int KS = D / 32;               // steps of the score product
   constexpr int DT = D / 16;               // 16-dim tiles of O
   constexpr int RB = D * 2;                // bytes of an LDS row
@@ -45,13 +50,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   constexpr int HALF = TK * RB;            // K's or V's half of a stage
   constexpr int GG = D * C::kBytes / 16;   // 16-byte pieces of a row in the cache
   constexpr int NL = TK * GG / kPaThreads; // pieces a thread carries, of K and of V
-  constexpr int SETS = Q8 && RT == 1 ? 2 : 1;  // tiles in flight in registers
   constexpr int KSW = GR - 1;              // granule swaps: K by key, V by key pairs
   constexpr int VSW = GR / 2 - 1;
   const atlas_paged_attn_t& p = a.p;
 
   __shared__ __attribute__((aligned(16))) char lds[2][2 * HALF];
-  constexpr int NSC = PAGE16 ? 4 : TK;     // scales of a tile: by 16 keys, or by key
+  constexpr int NSC = PAGE16 ? NT : TK;     // scales of a tile: by 16 keys, or by key
   __shared__ __attribute__((aligned(16))) float scale_lds[2][2][NSC];
   __shared__ int strange_lds[2];             // tile (+ 1) of the stage that holds such values
   __shared__ uint8_t up_lds[2][TK * D / 8];  // bits of V values that are +inf or NaN, by key and dim
@@ -130,55 +134,84 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const char* vbase = kbase + p.v_offset;
   const int ts = int(p.token_stride);
   const int page_size = p.page_size;
-  TilePages<Q8, 4> pages;
+  TilePages<Q8, NT> pages;
   pages.begin(a, r, h, lane);
 
-  auto key_of = [&](int c) __attribute__((always_inline)) { return (c < k.ca ? c : c - k.ca + k.cb) * TK; };
-  auto bounds = [&](int c, int& lo, int& hi) __attribute__((always_inline)) {
-    lo = c < k.ca ? 0 : k.lo;
-    hi = (c < k.ca ? k.prefix : k.hi) - 1;
+  auto key_of = [&](int c) __attribute__((always_inline)) {
+    return (c < k.ca * SUB ? c : c - k.ca * SUB + k.cb * SUB) * TK;
   };
-  typedef TilePages<Q8, 4> Tiles;
-  // first key of the lane's 16-key tile of tile c
-  auto lane_tile = [&](int c) __attribute__((always_inline)) {
+  auto bounds = [&](int c, int& lo, int& hi) __attribute__((always_inline)) {
+    lo = c < k.ca * SUB ? 0 : k.lo;
+    hi = (c < k.ca * SUB ? k.prefix : k.hi) - 1;
+  };
+  typedef TilePages<Q8, NT> Tiles;
+  // 64 / NT tiles make a window: lane l holds the offset of the first row of 16-key tile
+  // l % NT of its tile l / NT, and that page's scales.  A window is read at once, when
+  // its first tile is asked for, so that the loads of the key loop are all alike and
+  // a wait for one tile's rows is not a wait for the next one's page ids.
+  constexpr int WIN = 64 / NT;
+  int64_t win_rows = 0;
+  float win_ks = 0.f, win_vs = 0.f;
+  int win0 = 0, win1 = 0;
+  auto open_window = [&](int c, int end) __attribute__((always_inline)) {
+    win0 = c;
+    win1 = min(end, c + WIN);
+    const int mine = min(c + lane / NT, win1 - 1);
     int lo, hi;
-    bounds(c, lo, hi);
-    return Tiles::tile_key(key_of(c), lane & 3, lo, hi);
+    bounds(mine, lo, hi);
+    const int tile = Tiles::tile_key(key_of(mine), lane & (NT - 1), lo, hi);
+    const int id = pages.read_id(a, tile);
+    win_rows = pages.row_offset(a, id, tile);
+    if constexpr (Q8) {
+      const float* sc = p.kv_scales + int64_t(h) * p.scale_stride_head + pages.valid(id) * p.scale_stride_page;
+      win_ks = sc[0];
+      win_vs = sc[p.scale_stride_kv];
+    }
   };
   // Piece j of a thread: row (j * 256 + tid) / GG of the tile, piece tid % GG of it.
   const int piece = tid % GG, prow0 = tid / GG;
   constexpr int RSTEP = kPaThreads / GG;  // rows between a thread's pieces
+  static_assert(RSTEP % 16 == 0, "a thread's pieces have the same place in their 16-key tiles");
+  const uint32_t piece_at = uint32_t((prow0 & 15) * ts + piece * 16);
+  constexpr int KTH = kPaThreads / TK;  // threads per key
+  constexpr int SETS = 2;               // tiles in flight in registers
   struct Raw {
     w4 k[NL], v[NL];
-    float scales;    // of the 16-key tiles, as read
-    float ks, vs;    // other page sizes: those of key tid / 4
+    float ks, vs;  // scales of 16-key tile lane % NT; other page sizes: of key tid / KTH
   };
   // Keys outside [lo, hi) of the tile's part repeat its nearest key.
-  auto load = [&](Raw& x, int c, int64_t rows_at, float scale) __attribute__((always_inline)) {
+  auto load = [&](Raw& x, int c) __attribute__((always_inline)) {
     const int kb = key_of(c);
     int lo, hi;
     bounds(c, lo, hi);
+    const bool whole = (kb >= lo) & (kb + TK <= hi + 1);
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
       if constexpr (PAGE16) {
         // (a wave's rows of one piece lie in one 16-key tile)
         const int kt = (j * RSTEP + wave * (64 / GG)) >> 4;
-        const int64_t row0 = Tiles::tile_row(rows_at, kt);
-        const int tile = Tiles::tile_key(kb, kt, lo, hi);
-        const uint32_t off = uint32_t((key - tile) * ts + piece * 16);
+        const int64_t row0 = Tiles::tile_row(win_rows, (c - win0) * NT + kt);
+        uint32_t off = piece_at;
+        if (!whole) {
+          const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
+          off = uint32_t((key - Tiles::tile_key(kb, kt, lo, hi)) * ts + piece * 16);
+        }
         x.k[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
         x.v[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);
       } else {
+        const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
         const int slot = slot_of(a, key);
         const int64_t at = pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts + piece * 16;
         x.k[j] = *reinterpret_cast<const w4*>(kbase + at);
         x.v[j] = *reinterpret_cast<const w4*>(vbase + at);
       }
     }
-    x.scales = scale;
-    if constexpr (Q8 && !PAGE16) {
-      const int slot = slot_of(a, min(max(kb + (tid >> 2), lo), hi));
+    if constexpr (Q8 && PAGE16) {
+      const int from = ((c - win0) * NT + (lane & (NT - 1))) * 4;
+      x.ks = __uint_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_uint(win_ks)));
+      x.vs = __uint_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_uint(win_vs)));
+    } else if constexpr (Q8) {
+      const int slot = slot_of(a, min(max(kb + tid / KTH, lo), hi));
       const float* s = p.kv_scales + int64_t(h) * p.scale_stride_head + pages.valid(pages.ids[slot]) * p.scale_stride_page;
       x.ks = s[0];
       x.vs = s[p.scale_stride_kv];
@@ -207,7 +240,8 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     dn_lds[st][row * (D / 8) + gr] = uint8_t(dn);
     return v;
   };
-  auto store = [&](const Raw& x, int st, int c) __attribute__((always_inline)) {
+  auto store = [&](const Raw& x, auto st_tag, int c) __attribute__((always_inline)) {
+    constexpr int st = decltype(st_tag)::value;
     char* kd = lds[st];
     char* vd = lds[st] + HALF;
     frag vv[Q8 ? 2 * NL : NL];
@@ -218,33 +252,43 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         *reinterpret_cast<w4*>(kd + row * RB + ((piece ^ (row & KSW)) << 4)) = x.k[j];
         vv[j] = x.v[j];
       } else {
+        // (half of the pieces write their second granule first: eight lanes then write eight
+        // different residues of granules, which share no bank)
+        const bool swap = piece & (GG / 2);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          *reinterpret_cast<frag*>(kd + row * RB + (((2 * piece + e) ^ (row & KSW)) << 4)) =
-              C::keys8(x.k[j][2 * e], x.k[j][2 * e + 1]);
-          vv[2 * j + e] = C::keys8(x.v[j][2 * e], x.v[j][2 * e + 1]);
+          const bool second = swap != (e == 1);
+          *reinterpret_cast<frag*>(kd + row * RB + (((2 * piece + second) ^ (row & KSW)) << 4)) =
+              C::keys8(second ? x.k[j][2] : x.k[j][0], second ? x.k[j][3] : x.k[j][1]);
+          vv[2 * j + e] = C::keys8(second ? x.v[j][2] : x.v[j][0], second ? x.v[j][3] : x.v[j][1]);
         }
       }
     }
+    auto granule = [&](int j) __attribute__((always_inline)) {
+      return Q8 ? 2 * piece + int(bool(piece & (GG / 2)) != bool(j & 1)) : piece;
+    };
     if (KIND != kCacheInt8 && masked_tile(key_of(c))) {
       // (the marks of a tile are whole: every thread writes its part, whether it has some or not)
       uint32_t odd = 0;
 #pragma unroll
       for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j)
-        vv[j] = take_out(vv[j], st, (Q8 ? j >> 1 : j) * RSTEP + prow0, Q8 ? 2 * piece + (j & 1) : piece, odd);
+        vv[j] = take_out(vv[j], st, (Q8 ? j >> 1 : j) * RSTEP + prow0, granule(j), odd);
       if (odd) strange_lds[st] = c + 1;
     }
 #pragma unroll
     for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j) {
-      const int row = (Q8 ? j >> 1 : j) * RSTEP + prow0, gr = Q8 ? 2 * piece + (j & 1) : piece;
+      const int row = (Q8 ? j >> 1 : j) * RSTEP + prow0, gr = granule(j);
       *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = vv[j];
     }
     if constexpr (Q8 && PAGE16) {
-      if (tid < 8) scale_lds[st][tid >> 2][tid & 3] = x.scales;
+      if (tid < NT) {
+        scale_lds[st][0][tid] = x.ks;
+        scale_lds[st][1][tid] = x.vs;
+      }
     } else if constexpr (Q8) {
-      if ((tid & 3) == 0) {
-        scale_lds[st][0][tid >> 2] = x.ks;
-        scale_lds[st][1][tid >> 2] = x.vs;
+      if (tid % KTH == 0) {
+        scale_lds[st][0][tid / KTH] = x.ks;
+        scale_lds[st][1][tid / KTH] = x.vs;
       }
     }
   };
@@ -257,27 +301,24 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int vkey = 4 * g + e4;
 
   // One tile for this wave's row tiles, 32 keys at a time.
-  auto compute = [&](auto masked_tag, int st, int c) __attribute__((always_inline)) {
+  auto compute = [&](auto masked_tag, auto st_tag, int c) __attribute__((always_inline)) {
     constexpr bool masked = decltype(masked_tag)::value;
+    constexpr int st = decltype(st_tag)::value;
     const int kb = key_of(c);
     const char* kd = lds[st];
     const char* vd = lds[st] + HALF;
     const bool strange = masked && KIND != kCacheInt8 && strange_lds[st] == c + 1;
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
+    for (int hh = 0; hh < TK / 32; ++hh) {
       f32x4 acc[RT][2];
+      // The reads of an operand run ahead of the products before it, in this order: the
+      // compiler would put each next to its use, and every product would wait for its read.
+      frag kf[2][KS];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const frag kf = *reinterpret_cast<const frag*>(kd + (hh * 32 + kt * 16 + r16) * RB +
-                                                         (((ks * 4 + g) ^ (r16 & KSW)) << 4));
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) acc[rt][kt] = C::mfma(kf, qf[rt][ks], acc[rt][kt]);
-        }
-      }
+        for (int kt = 0; kt < 2; ++kt)
+          kf[kt][ks] = *reinterpret_cast<const frag*>(kd + (hh * 32 + kt * 16 + r16) * RB + (((ks * 4 + g) ^ (r16 & KSW)) << 4));
       f32x4 ksk[2], vsk[2];  // scales of the lane's keys (by 16-key tile: the first element)
       if constexpr (Q8) {
 #pragma unroll
@@ -290,10 +331,32 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
             vsk[kt] = *reinterpret_cast<const f32x4*>(&scale_lds[st][1][hh * 32 + kt * 16 + 4 * g]);
           }
         }
-        float top = fmaxf(vsk[0][0], vsk[1][0]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = C::mfma(kf[kt][ks], qf[rt][ks], acc[rt][kt]);
+      __builtin_amdgcn_sched_barrier(0);
+      frag vf[DT];  // V^T's operands by dim tile
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const char* at = vd + (32 * hh + vkey) * RB + (((2 * t + (q4 >> 1)) ^ ((vkey & VSW) << 1)) << 4) + ((q4 & 1) << 3);
+        const w2 lo = read_tr16(at), hi = read_tr16(at + 16 * RB);
+        vf[t] = frag{lo[0], lo[1], hi[0], hi[1]};
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (Q8) {
+        float top = pa_max(vsk[0][0], vsk[1][0]);
         if constexpr (!PAGE16) {
 #pragma unroll
-          for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(vsk[0][i], vsk[1][i]));
+          for (int i = 1; i < 4; ++i) top = pa_max(top, pa_max(vsk[0][i], vsk[1][i]));
           top = groups_max(top);
         }
         if (__builtin_amdgcn_ballot_w64(top > vref) != 0) {
@@ -336,26 +399,20 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
           }
           if (p.alibi_slopes != nullptr) {
             const float away = float(qpos - key0);
-            if (kb + TK <= shift + k.n0 + 1) {  // no key of the tile stands behind a query
-              const float b0 = -slope[rt] * away;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) x[i] += __builtin_fmaf(slope[rt], float((i >> 2) * 16 + (i & 3)), b0);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                x[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), x[i]);
-            }
+            for (int i = 0; i < 8; ++i)
+              x[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), x[i]);
           }
         }
         if constexpr (masked) {
           uint64_t w = 0;
           int w0 = col0;
           if (p.mask_mode == 1) {
-            // one word of the tree's columns, or one for each 64 keys (a tile is one of them)
+            // one word of the tree's columns, or one for each 64 keys (a tile lies in one of them)
             const int idx = p.mask_words > 1 ? (kb >> 6) - (col0 >> 6) : 0;
             if (idx >= 0 && idx < p.mask_words) w = p.tree_mask[int64_t(r.q0 + node_of[rt]) * p.mask_words + idx];
             if (idx < 0) w = ~0ull;
-            if (p.mask_words > 1) w0 = kb;
+            if (p.mask_words > 1) w0 = kb & ~63;
           }
           const int wlo = p.window_left >= 0 ? qpos - p.window_left : 0;
 #pragma unroll
@@ -405,14 +462,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         }
       }
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        // V^T's operand of dim tile t
-        const char* at = vd + (32 * hh + vkey) * RB + (((2 * t + (q4 >> 1)) ^ ((vkey & VSW) << 1)) << 4) + ((q4 & 1) << 3);
-        const w2 lo = read_tr16(at), hi = read_tr16(at + 16 * RB);
-        const frag vf = frag{lo[0], lo[1], hi[0], hi[1]};
+      for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf, pf[rt], o[rt][t]);
-      }
+        for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf[t], pf[rt], o[rt][t]);
       if (masked && strange) {
         // Where a row sees an infinity or NaN, its sum becomes one: a product with the
         // marks is zero for the rows that do not.
@@ -438,76 +490,46 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     }
   };
 
-  const int c0 = split * k.per, c1 = min(k.chunks, c0 + k.per);
+  const int c0 = split * k.per * SUB, c1 = min(k.chunks, (split + 1) * k.per) * SUB;
   if (c0 < c1) {
     if (tid < 2) strange_lds[tid] = 0;
-    // Ahead of the tile that is computed: one in LDS, SETS in registers, the scales
-    // of the one behind them, and the page ids of the next.
-    auto at = [&](int c) { return min(c, c1 - 1); };
-    int64_t rows_at = 0;
-    int id = 0;
-    float sc = 0.f;
+    // Ahead of the tile that is computed: one in LDS, SETS in registers.
     Raw x[SETS];
-    auto first_load = [&](Raw& y, int c) __attribute__((always_inline)) {
-      int64_t rows = 0;
-      float scale = 0.f;
+    auto ask = [&](Raw& y, int c) __attribute__((always_inline)) {
+      if (c >= c1) return;
       if constexpr (PAGE16) {
-        const int t = lane_tile(at(c)), i = pages.read_id(a, t);
-        rows = pages.row_offset(a, i, t);
-        scale = pages.read_scale(i);
+        if (c >= win1) open_window(c, c1);
       }
-      load(y, at(c), rows, scale);
+      load(y, c);
     };
-    first_load(x[0], c0);
+    if constexpr (PAGE16) open_window(c0, c1);
+    load(x[0], c0);
     lds_barrier();  // (the marks are cleared)
-    store(x[0], 0, c0);
+    store(x[0], Stage<0>{}, c0);
 #pragma unroll
-    for (int i = 0; i < SETS; ++i) first_load(x[i], c0 + 1 + i);
-    if constexpr (PAGE16) {
-      const int t = lane_tile(at(c0 + 1 + SETS)), i = pages.read_id(a, t);
-      rows_at = pages.row_offset(a, i, t);
-      sc = pages.read_scale(i);
-      id = pages.read_id(a, lane_tile(at(c0 + 2 + SETS)));
-    }
+    for (int i = 1; i <= SETS; ++i) ask(x[i % SETS], c0 + i);
     lds_barrier();
-    auto step = [&](auto masked_tag, Raw& y, int c) __attribute__((always_inline)) {
-      const int st = (c - c0) & 1;
+    auto step = [&](auto masked_tag, auto st_tag, Raw& y, int c) __attribute__((always_inline)) {
       // the next tile's registers go to the other stage, which every wave left
       // before the last barrier; then the one SETS behind it is asked for
-      if (c + 1 < c1) store(y, st ^ 1, c + 1);
-      int next_id = 0;
-      int64_t next_rows = 0;
-      float next_sc = 0.f;
-      if constexpr (PAGE16) {
-        next_id = pages.read_id(a, lane_tile(at(c + 3 + SETS)));
-        next_sc = pages.read_scale(id);
-        next_rows = pages.row_offset(a, id, lane_tile(at(c + 2 + SETS)));
-      }
-      if (c + 1 + SETS < c1) load(y, c + 1 + SETS, rows_at, sc);
-      id = next_id;
-      rows_at = next_rows;
-      sc = next_sc;
-      if (computes) compute(masked_tag, st, c);
+      if (c + 1 < c1) store(y, Stage<1 - decltype(st_tag)::value>{}, c + 1);
+      ask(y, c + 1 + SETS);
+      if (computes) compute(masked_tag, st_tag, c);
       lds_barrier();
     };
     // Runs of tiles without hidden keys take the shorter form.  (A choice at every tile
-    // would keep both forms' registers alive.)
+    // would keep both forms' registers alive.)  Stages and sets alternate, so tiles come in
+    // pairs and their addresses are constants.
+    auto masked_pair = [&](int c) { return masked_tile(key_of(c)) || (c + 1 < c1 && masked_tile(key_of(c + 1))); };
     int c = c0;
     while (c < c1) {
-      if constexpr (SETS == 1) {
-        for (; c < c1 && masked_tile(key_of(c)); ++c) step(std::true_type{}, x[0], c);
-        for (; c < c1 && !masked_tile(key_of(c)); ++c) step(std::false_type{}, x[0], c);
-      } else {
-        // (the sets alternate, so tiles come in pairs)
-        auto masked_pair = [&](int c) { return masked_tile(key_of(c)) || (c + 1 < c1 && masked_tile(key_of(c + 1))); };
-        for (; c < c1 && masked_pair(c); c += 2) {
-          step(std::true_type{}, x[0], c);
-          if (c + 1 < c1) step(std::true_type{}, x[SETS - 1], c + 1);
-        }
-        for (; c < c1 && !masked_pair(c); c += 2) {
-          step(std::false_type{}, x[0], c);
-          if (c + 1 < c1) step(std::false_type{}, x[SETS - 1], c + 1);
-        }
+      for (; c < c1 && masked_pair(c); c += 2) {
+        step(std::true_type{}, Stage<0>{}, x[1], c);
+        if (c + 1 < c1) step(std::true_type{}, Stage<1>{}, x[0], c + 1);
+      }
+      for (; c < c1 && !masked_pair(c); c += 2) {
+        step(std::false_type{}, Stage<0>{}, x[1], c);
+        if (c + 1 < c1) step(std::false_type{}, Stage<1>{}, x[0], c + 1);
       }
     }
   }
