@@ -117,6 +117,7 @@ __device__ __forceinline__ Block plan_block(const PagedAttnArgs& a, const Reques
   k.chunks = k.ca + (k.hi + kChunk - 1) / kChunk - k.cb;
   k.per = max(p.split_keys / kChunk, (k.chunks + p.num_splits - 1) / p.num_splits);
   k.splits = max(1, (k.chunks + k.per - 1) / k.per);
+  k.per = (k.chunks + k.splits - 1) / k.splits;  // (as equal as they come)
   return k;
 }
 

@@ -16,8 +16,11 @@ void launch_paged_kernel(const PagedAttnArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 1, PAGE16, SCORED, false>), grid, block, 0, stream, a);
   else if (p.block_rows <= 16)
     hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 1, PAGE16, SCORED, true>), grid, block, 0, stream, a);
-  else if (PAGE16 && p.block_rows <= 64)
-    hipLaunchKernelGGL((paged_rows_kernel<KIND, D, PAGE16 ? 1 : 2, PAGE16, SCORED>), grid, block, 0, stream, a);
+  else if (PAGE16 && p.block_rows <= 32)
+    hipLaunchKernelGGL((paged_stream_kernel<KIND, D, PAGE16 ? 2 : 1, PAGE16, SCORED, true>), grid, block, 0, stream, a);
+  else if (PAGE16 && Cache<KIND>::kQuant && p.block_rows <= 48)
+    hipLaunchKernelGGL((paged_stream_kernel<KIND, D, PAGE16 && Cache<KIND>::kQuant ? 3 : 1, PAGE16, SCORED, true>), grid,
+                       block, 0, stream, a);
   else
     hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 2, PAGE16, SCORED>), grid, block, 0, stream, a);
 }

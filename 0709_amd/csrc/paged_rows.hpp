@@ -28,6 +28,7 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+#define SETPRIO(x) __builtin_amdgcn_s_setprio(x)
 template <int N>
 using Stage = std::integral_constant<int, N>;
 
@@ -333,6 +334,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         }
       }
       __builtin_amdgcn_sched_barrier(0);
+      SETPRIO(1);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -343,6 +345,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = C::mfma(kf[kt][ks], qf[rt][ks], acc[rt][kt]);
+      SETPRIO(0);
       __builtin_amdgcn_sched_barrier(0);
       frag vf[DT];  // V^T's operands by dim tile
 #pragma unroll
@@ -461,10 +464,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
           pf[rt][kt * 2 + 1] = C::pack(e[2], e[3]);
         }
       }
+      SETPRIO(1);
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf[t], pf[rt], o[rt][t]);
+      SETPRIO(0);
       if (masked && strange) {
         // Where a row sees an infinity or NaN, its sum becomes one: a product with the
         // marks is zero for the rows that do not.

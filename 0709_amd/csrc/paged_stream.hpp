@@ -54,7 +54,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   constexpr int VW = VB / 4;
   constexpr int OS = D + 4;               // LDS row stride (floats)
   constexpr int NS = PAGE16 ? KT : KT * 4;  // scales of a step: by tile or by key
-  constexpr int NB = Q8 && PAGE16 && RT == 1 ? 3 : 2;  // steps in registers
+  constexpr int NB = RT > 1 ? 1 : 2;      // steps in registers
   constexpr bool QLDS = RT > 1;           // more than one tile of queries stays in LDS
   const atlas_paged_attn_t& p = a.p;
 
@@ -161,10 +161,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   TilePages<Q8, KT> pages;
   pages.begin(a, r, h, lane);
 
-  struct Raw {
+  struct RawK {
     uint32_t k[KT][KL * 4];
-    uint32_t v[KT][4][VW];
     float ks[NS], vs[NS];
+  };
+  struct RawV {
+    uint32_t v[KT][4][VW];
   };
   // first key of step s
   auto key_of = [&](int s) __attribute__((always_inline)) {
@@ -202,53 +204,34 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   const uint32_t k_lane = uint32_t(r16 * ts + g * 16), v_lane = uint32_t(4 * g * ts + r16 * VB);
   // Keys outside [lo, hi) of the step's part repeat its nearest key, so that
   // every load falls on a row that is there.
-  auto load = [&](Raw& x, int s) __attribute__((always_inline)) {
+  auto load_k = [&](RawK& x, int s) __attribute__((always_inline)) {
     const int kb = key_of(s);
     int lo, hi;
     bounds(s, lo, hi);
-    if constexpr (PAGE16) {
-      const bool whole = kb >= lo && kb + CK <= hi + 1;
+    const bool whole = (kb >= lo) & (kb + CK <= hi + 1);
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        // the tile's first row; then lane offsets from it
-        const int64_t row0 = Tiles::tile_row(win_rows, (s - win0) * KT + kt);
-        const char* kp = kbase + row0;
-        const char* vp = vbase + row0;
-        uint32_t ko = k_lane, vo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vo[i] = v_lane + uint32_t(i * ts);
-        if (!whole) {
-          const int t0 = kb + kt * 16, tile = Tiles::tile_key(kb, kt, lo, hi);
-          ko = uint32_t((min(max(t0 + r16, lo), hi) - tile) * ts + g * 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vo[i] = uint32_t((min(max(t0 + 4 * g + i, lo), hi) - tile) * ts + r16 * VB);
-        }
+    for (int kt = 0; kt < KT; ++kt) {
+      const int t0 = kb + kt * 16;
+      if constexpr (PAGE16) {
+        const char* kp = kbase + Tiles::tile_row(win_rows, (s - win0) * KT + kt);
+        uint32_t ko = k_lane;
+        if (!whole) ko = uint32_t((min(max(t0 + r16, lo), hi) - Tiles::tile_key(kb, kt, lo, hi)) * ts + g * 16);
 #pragma unroll
         for (int j = 0; j < KL; ++j) load_words<16>(kp + (ko + j * 64), &x.k[kt][4 * j]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_words<VB>(vp + vo[i], x.v[kt][i]);
         if constexpr (Q8) {
           x.ks[kt] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(win_ks), (s - win0) * KT + kt));
           x.vs[kt] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(win_vs), (s - win0) * KT + kt));
         }
-      }
-    } else {
-      auto page_of = [&](int slot) __attribute__((always_inline)) { return pages.valid(pages.ids[slot]); };
-#pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const int t0 = kb + kt * 16;
+      } else {
         const int key = min(max(t0 + r16, lo), hi);
         const int slot = slot_of(a, key);
-        const char* kp = kbase + page_of(slot) * p.page_stride + int64_t(key - slot * page_size) * ts;
+        const char* kp = kbase + pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts;
 #pragma unroll
         for (int j = 0; j < KL; ++j) load_words<16>(kp + j * 64 + g * 16, &x.k[kt][4 * j]);
+        if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int vk = min(max(t0 + 4 * g + i, lo), hi);
-          const int vslot = slot_of(a, vk);
-          const int64_t page = page_of(vslot);
-          load_words<VB>(vbase + page * p.page_stride + int64_t(vk - vslot * page_size) * ts + r16 * VB, x.v[kt][i]);
-          if constexpr (Q8) {
+          for (int i = 0; i < 4; ++i) {
+            const int64_t page = pages.valid(pages.ids[slot_of(a, min(max(t0 + 4 * g + i, lo), hi))]);
             const float* sc = p.kv_scales + int64_t(h) * p.scale_stride_head + page * p.scale_stride_page;
             x.ks[kt * 4 + i] = sc[0];
             x.vs[kt * 4 + i] = sc[p.scale_stride_kv];
@@ -257,14 +240,47 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
       }
     }
   };
+  auto load_v = [&](RawV& x, int s) __attribute__((always_inline)) {
+    const int kb = key_of(s);
+    int lo, hi;
+    bounds(s, lo, hi);
+    const bool whole = (kb >= lo) & (kb + CK <= hi + 1);
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int t0 = kb + kt * 16;
+      if constexpr (PAGE16) {
+        const char* vp = vbase + Tiles::tile_row(win_rows, (s - win0) * KT + kt);
+        uint32_t vo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vo[i] = v_lane + uint32_t(i * ts);
+        if (!whole) {
+          const int tile = Tiles::tile_key(kb, kt, lo, hi);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vo[i] = uint32_t((min(max(t0 + 4 * g + i, lo), hi) - tile) * ts + r16 * VB);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load_words<VB>(vp + vo[i], x.v[kt][i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = min(max(t0 + 4 * g + i, lo), hi);
+          const int slot = slot_of(a, key);
+          load_words<VB>(vbase + pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts + r16 * VB,
+                         x.v[kt][i]);
+        }
+      }
+    }
+  };
 
   // Largest V scale so far: O holds sums of p * v * (scale / vref).
   float vref = 1.17549435e-38f, vinv = 8.5070592e37f;
 
-  auto compute = [&](const Raw& x, int s) __attribute__((always_inline)) {
+  auto masked_step = [&](int s) __attribute__((always_inline)) {
     const int kb = key_of(s);
-    const bool masked = ((kb + CK > plain_hi) | (kb < plain_lo)) & (kb + CK > k.prefix);
-    f32x4 acc[RT][KT];
+    return ((kb + CK > plain_hi) | (kb < plain_lo)) & (kb + CK > k.prefix);
+  };
+  f32x4 acc[RT][KT];
+  auto scores = [&](const RawK& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -284,10 +300,16 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
         for (int kt = 0; kt < KT; ++kt) acc[rt][kt] = C::mfma(kf[kt], q, acc[rt][kt]);
       }
     }
+  };
+  // The softmax's part: weights pf of the step's scores (ks, vs: its scales).
+  frag pf[RT][KT / 2];
+  auto weights = [&](auto masked_tag, int s, const float (&ks_of)[NS], const float (&vs_of)[NS]) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(masked_tag)::value;
+    const int kb = key_of(s);
     if constexpr (Q8) {
-      float top = x.vs[0];
+      float top = vs_of[0];
 #pragma unroll
-      for (int i = 1; i < NS; ++i) top = fmaxf(top, x.vs[i]);
+      for (int i = 1; i < NS; ++i) top = pa_max(top, vs_of[i]);
       if (__builtin_amdgcn_ballot_w64(top > vref) != 0) {
         if constexpr (!PAGE16) top = groups_max(top);
         const float now = fmaxf(vref, top);
@@ -301,13 +323,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
       }
     }
     const int key0 = kb + 4 * g;
-    frag pf[RT][KT / 2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float sc[KT * 4];
 #pragma unroll
       for (int i = 0; i < KT * 4; ++i)
-        sc[i] = acc[rt][i >> 2][i & 3] * (Q8 ? qscale[rt] * x.ks[PAGE16 ? i >> 2 : i] : qscale[rt]);
+        sc[i] = acc[rt][i >> 2][i & 3] * (Q8 ? qscale[rt] * ks_of[PAGE16 ? i >> 2 : i] : qscale[rt]);
       if (SCORED && p.soft_cap > 0.f) {
         // cap * tanh(y / cap) = cap * (1 - 2 / (1 + e^(2 y / cap))), to powers of two
 #pragma unroll
@@ -322,7 +343,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
         for (int i = 0; i < KT * 4; ++i)
           sc[i] = __builtin_fmaf(-slope[rt], fabsf(away - float((i >> 2) * 16 + (i & 3))), sc[i]);
       }
-      if (masked) {
+      if constexpr (masked) {
         uint64_t w = 0;
         int w0 = col0;
         if (MULTI && p.mask_mode == 1) {
@@ -367,36 +388,40 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
         for (int i = 0; i < 4; ++i) {
           e[i] = __builtin_amdgcn_exp2f(sc[kt * 4 + i] - m);
           l_run[rt] += e[i];
-          if constexpr (Q8) e[i] *= x.vs[PAGE16 ? kt : kt * 4 + i] * vinv;
+          if constexpr (Q8) e[i] *= vs_of[PAGE16 ? kt : kt * 4 + i] * vinv;
         }
         pf[rt][kt >> 1][(kt & 1) * 2] = C::pack(e[0], e[1]);
         pf[rt][kt >> 1][(kt & 1) * 2 + 1] = C::pack(e[2], e[3]);
       }
     }
+  };
+  auto values = [&](auto masked_tag, const RawV& x) __attribute__((always_inline)) {
+    constexpr bool masked = decltype(masked_tag)::value;
 #pragma unroll
-    for (int tp = 0; tp < KT / 2; ++tp) {
-      uint32_t raw[8][VW];
+    for (int tp = 0; tp < KT / 2; ++tp)
+      // (a word of each row at a time: its dims' operands are all that is alive)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int w = 0; w < VW; ++w) {
+        constexpr int DW = DL / VW;
+        uint32_t raw[8][1];
 #pragma unroll
-        for (int w = 0; w < VW; ++w) raw[i][w] = x.v[2 * tp + (i >> 2)][i & 3][w];
-      frag vf[DL];
-      transpose_v<KIND, VW, DL>(raw, vf);
-      if constexpr (MULTI && KIND != kCacheInt8) {
-        // Infinities and NaN in V rows that a row does not see must not reach it
-        // (0 * inf): where keys are hidden they are taken out of the product, and the
-        // rows that see them get them from a product with their marks.
-        if (masked) {
+        for (int i = 0; i < 8; ++i) raw[i][0] = x.v[2 * tp + (i >> 2)][i & 3][w];
+        frag vf[DW];
+        transpose_v<KIND, 1, DW>(raw, vf);
+        if constexpr (MULTI && masked && KIND != kCacheInt8) {
+          // Infinities and NaN in V rows that a row does not see must not reach it
+          // (0 * inf): where keys are hidden they are taken out of the product, and the
+          // rows that see them get them from a product with their marks.
           uint32_t odd = 0;
 #pragma unroll
-          for (int t = 0; t < DL; ++t)
+          for (int t = 0; t < DW; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) odd |= not_finite2<C::kBf16>(vf[t][j]);
           if (__builtin_amdgcn_ballot_w64(odd != 0) != 0) {
             constexpr uint32_t kOne = C::kBf16 ? 0x3f80u : 0x3c00u;
             constexpr float kHuge = 3e38f;
 #pragma unroll
-            for (int t = 0; t < DL; ++t) {
+            for (int t = 0; t < DW; ++t) {
               frag up, dn;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -409,37 +434,76 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
               for (int rt = 0; rt < RT; ++rt) {
                 const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
                 const f32x4 plus = C::mfma(up, pf[rt][tp], zero), minus = C::mfma(dn, pf[rt][tp], zero);
-                o[rt][t] += plus * kHuge * kHuge - minus * kHuge * kHuge;
+                o[rt][w * DW + t] += plus * kHuge * kHuge - minus * kHuge * kHuge;
               }
             }
           }
         }
+#pragma unroll
+        for (int t = 0; t < DW; ++t)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][w * DW + t] = C::mfma(vf[t], pf[rt][tp], o[rt][w * DW + t]);
       }
-#pragma unroll
-      for (int t = 0; t < DL; ++t)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf[t], pf[rt][tp], o[rt][t]);
-    }
   };
 
-  // NB - 1 steps are in flight while one is computed; past the window's last step it is
-  // asked for again rather than branched around, so the waits stay exact.
   for (int s = s0; s < s1;) {
     const int end = PAGE16 ? min(s1, s + WIN) : s1;
     if constexpr (PAGE16) open_window(s, end);
-    Raw x[NB];
+    auto at = [&](int t) { return min(t, end - 1); };
+    if constexpr (NB > 1) {
+      // NB - 1 steps are in flight while one is computed; past the window's last step it
+      // is asked for again rather than branched around, so the waits stay exact.
+      RawK xk[NB];
+      RawV xv[NB];
 #pragma unroll
-    for (int i = 0; i < NB - 1; ++i) load(x[i], min(s + i, end - 1));
-    auto step = [&](Raw& cur, Raw& last) __attribute__((always_inline)) {
-      load(last, min(s + NB - 1, end - 1));
-      compute(cur, s);
-      return ++s < end;
-    };
-    if constexpr (NB == 2) {
-      while (step(x[0], x[1]) && step(x[1], x[0])) {
+      for (int i = 0; i < NB - 1; ++i) {
+        load_k(xk[i], at(s + i));
+        load_v(xv[i], at(s + i));
+      }
+      auto step = [&](int cur, int last) __attribute__((always_inline)) {
+        load_k(xk[last], at(s + NB - 1));
+        load_v(xv[last], at(s + NB - 1));
+        scores(xk[cur]);
+        if (masked_step(s)) {
+          weights(std::true_type{}, s, xk[cur].ks, xk[cur].vs);
+          values(std::true_type{}, xv[cur]);
+        } else {
+          weights(std::false_type{}, s, xk[cur].ks, xk[cur].vs);
+          values(std::false_type{}, xv[cur]);
+        }
+        return ++s < end;
+      };
+      if constexpr (NB == 2) {
+        while (step(0, 1) && step(1, 0)) {
+        }
+      } else {
+        while (step(0, 2) && step(1, 0) && step(2, 1)) {
+        }
       }
     } else {
-      while (step(x[0], x[NB - 1]) && step(x[1], x[0]) && step(x[NB - 1], x[1])) {
+      // The rows of O leave room for one step: the next step's K is asked for when the
+      // scores are done with this one's, its V when the second product is.
+      RawK xk;
+      RawV xv;
+      load_k(xk, s);
+      load_v(xv, s);
+      auto step = [&](auto masked_tag) __attribute__((always_inline)) {
+        scores(xk);
+        float ks_of[NS], vs_of[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          ks_of[i] = xk.ks[i];
+          vs_of[i] = xk.vs[i];
+        }
+        load_k(xk, at(s + 1));
+        weights(masked_tag, s, ks_of, vs_of);
+        values(masked_tag, xv);
+        load_v(xv, at(s + 1));
+        ++s;
+      };
+      while (s < end) {
+        while (s < end && masked_step(s)) step(std::true_type{});
+        while (s < end && !masked_step(s)) step(std::false_type{});
       }
     }
   }

@@ -33,18 +33,22 @@ from . import _lib
 from .tree_attention import _host_lists
 
 # Most packed query rows (query token * group + head of the group) of a workgroup:
-# the kernel of few rows, and that of many rows with one and with two row tiles a wave.
-STREAM_ROWS = 16
-NARROW_ROWS = 64
+# one token per request; few rows, over 8-bit caches, over 16-bit ones, and where the page
+# size is no multiple of 16; many rows.
+DECODE_ROWS = 16
+STREAM_ROWS_8BIT = 48
+STREAM_ROWS_16BIT = 32
+STREAM_ROWS_PAGES = 16
 WIDE_ROWS = 128
-# Requests of more packed rows than this take the wide blocks.
-MAX_NARROW_ROWS = 192
+# Requests of more packed rows than this take the kernel of many rows.
+MAX_STREAM_ROWS = 192
 # Workgroups to aim for when the keys are split, and the least keys of a split.
 # Decode splits are never longer than MAX_DECODE_SPLIT keys where the batch is
 # large: short splits even out requests of different lengths.
 DECODE_WORKGROUPS = 1024
 MAX_DECODE_SPLIT = 1536
-BLOCK_WORKGROUPS = 512
+STREAM_WORKGROUPS = 512
+BLOCK_WORKGROUPS = 1024
 MIN_SPLIT_KEYS = 256
 MAX_SPLITS = 256
 
@@ -55,7 +59,7 @@ _ARGS = struct.Struct("=14Q15q15i2f4x")
 
 
 def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int, *, tree: bool = False,
-                 page_size: int = 16) -> tuple[bool, int, int, int, int]:
+                 quantized: bool = False, page_size: int = 16) -> tuple[bool, int, int, int, int]:
     """(single token?, rows of a block, row blocks, splits, keys per split) of a call.
 
     One query token per request takes blocks of 16 packed rows, more take equal
@@ -64,10 +68,11 @@ def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_l
     ``max_kv_len`` takes fewer splits of the same size."""
     single = max_q_len <= 1 and not tree
     rows = max(1, max_q_len * group)
-    if single or rows <= STREAM_ROWS:
-        most_rows, target = STREAM_ROWS, DECODE_WORKGROUPS
-    elif rows <= MAX_NARROW_ROWS and page_size % 16 == 0:
-        most_rows, target = NARROW_ROWS, BLOCK_WORKGROUPS
+    if single:
+        most_rows, target = DECODE_ROWS, DECODE_WORKGROUPS
+    elif rows <= MAX_STREAM_ROWS:
+        most_rows = STREAM_ROWS_PAGES if page_size % 16 else (STREAM_ROWS_8BIT if quantized else STREAM_ROWS_16BIT)
+        target = STREAM_WORKGROUPS
     else:
         most_rows, target = WIDE_ROWS, BLOCK_WORKGROUPS
     blocks = -(-rows // most_rows)
@@ -256,7 +261,7 @@ def paged_attention(
     # (keys that a window leaves to a row block; the visible prefix comes on top)
     reach = max_kv_len if window_left < 0 or prefix_lens is not None else min(max_kv_len, window_left + max_q_len)
     shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach), tree=mode == _lib.MASK_TREE,
-                         page_size=page_size)
+                         quantized=s is not None, page_size=page_size)
     need = workspace_bytes(batch, hkv, d, shape)
     if need:
         if workspace is None:
