@@ -15,6 +15,8 @@ typedef uint32_t w2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr int kAppendThreads = 256;
+constexpr int kHeld = 8;  // vectors of a thread's rows in registers
+constexpr int kCommitWaves = 4;
 
 struct QuantTables {
   char* kv[ATLAS_MAX_LAYERS_PER_LAUNCH];
@@ -58,8 +60,21 @@ __device__ __forceinline__ void to_floats(w4 v, float (&f)[8]) {
   }
 }
 
+// Four codes under a scale that is 1 / ratio times theirs.
+template <int CACHE>
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+  float f[4];
+  Quant8<CACHE>::decode4(w, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f[e] *= ratio;
+  return Quant8<CACHE>::encode4(f);
+}
+
 // One unit (a touched page's rows of one head, K or V, of one layer) per UNIT
-// threads.  Two passes over the unit's new rows: their largest value, then the codes.
+// threads: the rows are read once, into registers (kHeld vectors of 8 values a
+// thread; what a large page holds beyond that is read twice), their largest value
+// gives the scale, and the codes follow.  Bound by the bytes: 2 read and 1 written
+// per value.
 template <int CACHE, bool BF16, int UNIT>
 __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(QuantTables qt, RowTables st, QuantGeom g,
                                                                              Appends a) {
@@ -97,22 +112,34 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(Qua
   live = live && page >= 0 && page < g.num_pages;
   const int o0 = int(max(first, p0) - p0);                       // first new row's place in the page
   const int o1 = live ? int(min(hi - p0, int64_t(g.page_size))) : o0;  // behind the last
-  const int vpr = g.head_dim / 8;  // vectors of 8 values per row
-  const int nvec = (o1 - o0) * vpr;
+  const int vs = g.head_dim == 64 ? 3 : 4, vmask = (1 << vs) - 1;  // vectors of 8 values per row
+  const int nvec = (o1 - o0) << vs;
 
   const char* src = (kv ? st.v[layer] : st.k[layer]) + ((r0 + p0 + o0 - lo) * a.src_stride + int64_t(head) * g.head_dim) * 2;
   char* dst = qt.kv[layer] + page * g.page_stride + kv * g.v_offset + int64_t(head) * g.head_stride;
   float* scale = qt.scales[layer] + page * g.scale_page + kv * g.scale_kv + head * g.scale_head;
   const float before = live ? *scale : 0.f;
 
-  float top = 0.f;
-  for (int i = t; i < nvec; i += UNIT) {
-    const int row = i / vpr, v = i - row * vpr;
-    float f[8];
-    to_floats<BF16>(*reinterpret_cast<const w4*>(src + (row * a.src_stride + v * 8) * 2), f);
+  auto read = [&](int i) __attribute__((always_inline)) {
+    return *reinterpret_cast<const w4*>(src + ((i >> vs) * a.src_stride + (i & vmask) * 8) * 2);
+  };
+  auto largest = [](w4 v) __attribute__((always_inline)) {
+    float f[8], m = 0.f;
+    to_floats<BF16>(v, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
+    return m;
+  };
+  float top = 0.f;
+  w4 held[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    held[k] = w4{0, 0, 0, 0};
+    if (t + k * UNIT < nvec) held[k] = read(t + k * UNIT);
   }
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) top = fmaxf(top, largest(held[k]));
+  for (int i = t + kHeld * UNIT; i < nvec; i += UNIT) top = fmaxf(top, largest(read(i)));
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
   if (UNIT > 64) {
@@ -127,25 +154,17 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(Qua
   // older rows, when the scale grew
   if (live && o0 > 0 && now != before) {
     const float ratio = before * up;
-    for (int i = t; i < o0 * vpr; i += UNIT) {
-      const int row = i / vpr, v = i - row * vpr;
-      w2* at = reinterpret_cast<w2*>(dst + row * g.token_stride + v * 8);
+    for (int i = t; i < o0 << vs; i += UNIT) {
+      w2* at = reinterpret_cast<w2*>(dst + (i >> vs) * g.token_stride + (i & vmask) * 8);
       w2 w = *at;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float f[4];
-        Q::decode4(w[j], f);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] *= ratio;
-        w[j] = Q::encode4(f);
-      }
+      w[0] = rescale4<CACHE>(w[0], ratio);
+      w[1] = rescale4<CACHE>(w[1], ratio);
       *at = w;
     }
   }
-  for (int i = t; i < nvec; i += UNIT) {
-    const int row = i / vpr, v = i - row * vpr;
+  auto write = [&](int i, w4 v) __attribute__((always_inline)) {
     float f[8];
-    to_floats<BF16>(*reinterpret_cast<const w4*>(src + (row * a.src_stride + v * 8) * 2), f);
+    to_floats<BF16>(v, f);
     w2 w;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -154,8 +173,12 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(Qua
       for (int e = 0; e < 4; ++e) x[e] = f[4 * j + e] * up;
       w[j] = Q::encode4(x);
     }
-    *reinterpret_cast<w2*>(dst + (o0 + row) * g.token_stride + v * 8) = w;
-  }
+    *reinterpret_cast<w2*>(dst + (o0 + (i >> vs)) * g.token_stride + (i & vmask) * 8) = w;
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (t + k * UNIT < nvec) write(t + k * UNIT, held[k]);
+  for (int i = t + kHeld * UNIT; i < nvec; i += UNIT) write(i, read(i));
   if (live && t == 0) *scale = now;
 }
 
@@ -169,97 +192,112 @@ struct Commits {
   int batch, max_items, layers;
 };
 
-// One wave per (layer, request, K or V, head): all of a request's rows of a head are
-// read into LDS before any is written, so sources and destinations may overlap.
-// Lane i prepares item i: its rows' offsets, its destination block's scales, and
-// whether it is the first item of that block.
-template <int CACHE>
-__global__ __launch_bounds__(64) void kv_commit_quantized_kernel(QuantTables qt, QuantGeom g, Commits c) {
-  typedef Quant8<CACHE> Q;
-  constexpr int kMax = ATLAS_QUANT_COMMIT_MAX_ITEMS;
-  __shared__ __attribute__((aligned(16))) uint32_t rows[kMax * 32];
-  __shared__ int64_t page_of[kMax], src_off[kMax], dst_off[kMax];
-  __shared__ float old_scale[kMax], src_scale[kMax], new_scale[kMax];
-  __shared__ int state[kMax];  // 0: skipped, 1: moved, 2: moved and first of its block
+__device__ __forceinline__ int64_t shuffle64(int64_t v, int lane) {
+  const uint32_t low = __shfl(uint32_t(v), lane), high = __shfl(uint32_t(v >> 32), lane);
+  return int64_t(uint64_t(high) << 32 | low);
+}
+
+// One wave per (layer, request, K or V, head).  All of a request's rows of a head are
+// read into registers before any is written, so sources and destinations may overlap.
+// Lane i holds item i: its rows' offsets, its blocks' scales, whether it is the first
+// item of its destination block; what the others need of it goes through readlane and
+// shuffles.  A few hundred bytes per wave: bound by the chain of loads from the
+// positions to the rows, so every wave of a call should be in flight at once.
+template <int CACHE, int D>
+__global__ __launch_bounds__(64 * kCommitWaves) void kv_commit_quantized_kernel(QuantTables qt, QuantGeom g, Commits c) {
+  constexpr int kLanes = D / 16;        // lanes of 16 codes per row
+  constexpr int kRows = 64 / kLanes;    // rows per pass
+  constexpr int kPasses = ATLAS_QUANT_COMMIT_MAX_ITEMS / kRows;
+  const int units = 2 * g.heads, groups = (units + kCommitWaves - 1) / kCommitWaves;
   int u = blockIdx.x;
-  const int head = u % g.heads;
-  u /= g.heads;
-  const int kv = u & 1;
-  u >>= 1;
+  const int unit = (u % groups) * kCommitWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  u /= groups;
   const int b = u % c.batch;
   const int layer = u / c.batch;
-  const int lane = threadIdx.x;
+  const int kv = unit >= g.heads, head = unit - kv * g.heads;
+  const int lane = threadIdx.x & 63;
 
   const int64_t i0 = min(max(int64_t(c.indptr[b]), int64_t(0)), c.num_items);
   const int64_t i1 = min(max(int64_t(c.indptr[b + 1]), i0), c.num_items);
-  const int n = int(min(i1 - i0, int64_t(c.max_items)));
-  if (n == 0) return;
+  // (a wave past the last unit moves nothing, but meets the others at the barriers)
+  const int n = unit < units ? int(min(i1 - i0, int64_t(c.max_items))) : 0;
   const int64_t pt = min(max(int64_t(c.kv_indptr[b]), int64_t(0)), g.num_indices);
   const int64_t np = min(max(int64_t(c.kv_indptr[b + 1]), pt), g.num_indices) - pt;
 
   char* base = qt.kv[layer] + kv * g.v_offset + int64_t(head) * g.head_stride;
   float* sbase = qt.scales[layer] + kv * g.scale_kv + head * g.scale_head;
-  auto place = [&](int64_t pos, int64_t& page, int64_t& off) {
+  auto place = [&](int64_t pos, int& page, int64_t& off) __attribute__((always_inline)) {
     const int64_t lp = g.page_shift >= 0 ? pos >> g.page_shift : pos / g.page_size;
     if (pos < 0 || lp >= np) return false;
     page = c.kv_indices[pt + lp];
     off = page * g.page_stride + (pos - lp * g.page_size) * g.token_stride;
     return page >= 0 && page < g.num_pages;
   };
+  int src_page = -1, page = -1;
+  int64_t src = 0, dst = 0;
+  float src_scale = 0.f, before = 0.f;
+  bool moves = false;
   if (lane < n) {
-    int64_t sp = 0, dp = 0, so = 0, dof = 0;
-    const bool ok = place(c.src_pos[i0 + lane], sp, so) && place(c.dst_pos[i0 + lane], dp, dof);
-    page_of[lane] = ok ? dp : -1;
-    src_off[lane] = so;
-    dst_off[lane] = dof;
-    src_scale[lane] = ok ? sbase[sp * g.scale_page] : 0.f;
-    old_scale[lane] = ok ? sbase[dp * g.scale_page] : 0.f;
-    state[lane] = ok;
-  }
-  __syncthreads();
-  if (lane < n && state[lane]) {
-    float now = old_scale[lane];
-    bool leads = true;
-    for (int j = 0; j < n; ++j) {
-      if (page_of[j] != page_of[lane]) continue;
-      now = fmaxf(now, src_scale[j]);
-      if (j < lane) leads = false;
+    const int64_t from = c.src_pos[i0 + lane], to = c.dst_pos[i0 + lane];
+    const bool from_ok = place(from, src_page, src), to_ok = place(to, page, dst);
+    moves = from_ok && to_ok;
+    if (moves) {
+      src_scale = sbase[src_page * g.scale_page];
+      before = sbase[page * g.scale_page];
     }
-    new_scale[lane] = now;
-    if (leads) state[lane] = 2;
   }
-  __syncthreads();
-  const int wpr = g.head_dim / 4;  // words per row
-  for (int i = lane; i < n * wpr; i += 64) {
-    const int item = i / wpr, w = i - item * wpr;
-    if (state[item]) rows[i] = *reinterpret_cast<const uint32_t*>(base + src_off[item] + w * 4);
+  if (!moves) page = -1;
+
+  w4 rows[kPasses];
+  const int word = (lane % kLanes) * 16;
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    if (k * kRows >= n) break;  // (the same for the wave: every lane takes part in the shuffles)
+    const int item = k * kRows + lane / kLanes;
+    const int64_t off = shuffle64(src, item);
+    if (__shfl(page, item) >= 0) rows[k] = *reinterpret_cast<const w4*>(base + off + word);
   }
-  __syncthreads();
+  // the block's new scale, its first item, and items whose row a later one writes again
+  float now = before;
+  bool leads = moves, stays = false;
   for (int j = 0; j < n; ++j) {
-    if (state[j] != 2 || new_scale[j] == old_scale[j]) continue;
-    const float ratio = old_scale[j] / new_scale[j];
-    char* page = base + page_of[j] * g.page_stride;
-    for (int i = lane; i < g.page_size * wpr; i += 64) {
-      const int row = i / wpr, w = i - row * wpr;
-      uint32_t* at = reinterpret_cast<uint32_t*>(page + row * g.token_stride + w * 4);
-      float f[4];
-      Q::decode4(*at, f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] *= ratio;
-      *at = Q::encode4(f);
-    }
-    if (lane == 0) sbase[page_of[j] * g.scale_page] = new_scale[j];
+    const int pj = __builtin_amdgcn_readlane(page, j);
+    const float sj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(src_scale), j));
+    if (pj < 0 || pj != page) continue;
+    now = fmaxf(now, sj);
+    if (j < lane) leads = false;
+    const int64_t dj = int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(dst >> 32), j))) << 32 |
+                               uint32_t(__builtin_amdgcn_readlane(int(dst), j)));
+    if (j > lane && dj == dst) stays = true;
   }
-  __syncthreads();  // (the rounded rows are in memory before rows are moved over them)
-  for (int i = lane; i < n * wpr; i += 64) {
-    const int item = i / wpr, w = i - item * wpr;
-    if (!state[item]) continue;
-    const float ratio = src_scale[item] / new_scale[item];
-    float f[4];
-    Q::decode4(rows[i], f);
+  __syncthreads();  // (every row has been read)
+  for (uint64_t grown = __ballot(leads && now != before); grown; grown &= grown - 1) {
+    const int j = __builtin_ctzll(grown);
+    const float ratio = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(before), j)) /
+                        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(now), j));
+    char* at = base + int64_t(__builtin_amdgcn_readlane(page, j)) * g.page_stride + word;
+    for (int row = lane / kLanes; row < g.page_size; row += kRows) {
+      w4* p = reinterpret_cast<w4*>(at + row * g.token_stride);
+      w4 w = *p;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] *= ratio;
-    *reinterpret_cast<uint32_t*>(base + dst_off[item] + w * 4) = Q::encode4(f);
+      for (int e = 0; e < 4; ++e) w[e] = rescale4<CACHE>(w[e], ratio);
+      *p = w;
+    }
+  }
+  if (leads && now != before) sbase[page * g.scale_page] = now;
+  __syncthreads();  // (the rounded rows are in memory before rows are moved over them)
+  const float ratio = src_scale / now;
+#pragma unroll
+  for (int k = 0; k < kPasses; ++k) {
+    if (k * kRows >= n) break;
+    const int item = k * kRows + lane / kLanes;
+    const int64_t off = shuffle64(dst, item);
+    const float r = __shfl(ratio, item);
+    if (!__shfl(int(moves && !stays), item)) continue;
+    w4 w = rows[k];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = rescale4<CACHE>(w[e], r);
+    *reinterpret_cast<w4*>(base + off + word) = w;
   }
 }
 
@@ -303,6 +341,12 @@ void launch_append(int64_t units, int unit, hipStream_t stream, const QuantTable
     hipLaunchKernelGGL((kv_append_quantized_kernel<CACHE, BF16, 64>), grid, dim3(kAppendThreads), 0, stream, qt, st, g, a);
   else
     hipLaunchKernelGGL((kv_append_quantized_kernel<CACHE, BF16, 256>), grid, dim3(kAppendThreads), 0, stream, qt, st, g, a);
+}
+
+template <int CACHE, int D>
+void launch_commit(int64_t blocks, hipStream_t stream, const QuantTables& qt, const QuantGeom& g, const Commits& c) {
+  hipLaunchKernelGGL((kv_commit_quantized_kernel<CACHE, D>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kCommitWaves),
+                     0, stream, qt, g, c);
 }
 
 }  // namespace
@@ -393,18 +437,19 @@ extern "C" int atlas_kv_commit_quantized(
     QuantTables qt;
     fill_quant_tables(qt, layers, scales, l0, nl);
     c.layers = nl;
-    const int64_t units = int64_t(nl) * batch * 2 * num_kv_heads;
-    if (units >= (int64_t(1) << 26)) {
+    const int64_t units = int64_t(nl) * batch * ((2 * int64_t(num_kv_heads) + kCommitWaves - 1) / kCommitWaves);
+    if (units >= (int64_t(1) << 24)) {
       set_error("%lld blocks are too many for one commit", static_cast<long long>(units));
       return ATLAS_EUNSUPPORTED;
     }
-    const dim3 grid(static_cast<unsigned>(units));
-    if (cache == ATLAS_CACHE_E4M3)
-      hipLaunchKernelGGL((kv_commit_quantized_kernel<ATLAS_CACHE_E4M3>), grid, dim3(64), 0,
-                         static_cast<hipStream_t>(stream), qt, g, c);
-    else
-      hipLaunchKernelGGL((kv_commit_quantized_kernel<ATLAS_CACHE_INT8>), grid, dim3(64), 0,
-                         static_cast<hipStream_t>(stream), qt, g, c);
+    const hipStream_t hs = static_cast<hipStream_t>(stream);
+    if (cache == ATLAS_CACHE_E4M3) {
+      if (head_dim == 128) launch_commit<ATLAS_CACHE_E4M3, 128>(units, hs, qt, g, c);
+      else launch_commit<ATLAS_CACHE_E4M3, 64>(units, hs, qt, g, c);
+    } else {
+      if (head_dim == 128) launch_commit<ATLAS_CACHE_INT8, 128>(units, hs, qt, g, c);
+      else launch_commit<ATLAS_CACHE_INT8, 64>(units, hs, qt, g, c);
+    }
     if ((rc = launch_status("kv_commit_quantized_kernel"))) return rc;
   }
   return ATLAS_OK;

@@ -22,6 +22,8 @@ of its last scale.
 
 from __future__ import annotations
 
+import ctypes
+from operator import attrgetter
 from typing import Sequence
 
 import torch
@@ -44,6 +46,26 @@ def alloc_quantized_layers(num_layers: int, num_pages: int, page_size: int, num_
     return list(codes.unbind(0)), list(scales.unbind(0))
 
 
+_dtype = attrgetter("dtype")
+
+
+def _alike(tensors: Sequence[torch.Tensor], first: torch.Tensor) -> bool:
+    """Whether all have ``first``'s shape, strides, dtype and (HIP) device."""
+    if len(tensors) == 1 and tensors[0] is first:
+        return True
+    # (dense tensors of one shape have the same strides wherever those matter)
+    dense = first.is_contiguous()
+    return (set(map(torch.Tensor.size, tensors)) == {first.shape}
+            and (all(map(torch.Tensor.is_contiguous, tensors)) if dense
+                 else set(map(torch.Tensor.stride, tensors)) == {first.stride()})
+            and set(map(_dtype, tensors)) == {first.dtype}
+            and set(map(torch.Tensor.get_device, tensors)) == {first.get_device()})
+
+
+def _pointers(tensors: Sequence[torch.Tensor]):
+    return (ctypes.c_void_p * len(tensors))(*map(torch.Tensor.data_ptr, tensors))
+
+
 def _check_layers(layers: Sequence[torch.Tensor], scales: Sequence[torch.Tensor], kv_layout: str, what: str):
     """The device and the arguments that describe the layers."""
     if not layers or len(scales) != len(layers):
@@ -53,17 +75,13 @@ def _check_layers(layers: Sequence[torch.Tensor], scales: Sequence[torch.Tensor]
     device = _lib.require_device(first, s0, what=what)
     if first.dtype not in CACHE_CODES:
         raise TypeError(f"{what} writes float8_e4m3fn or int8 layers, not {first.dtype}")
-    shape, stride, dtype = first.shape, first.stride(), first.dtype
-    for t in layers[1:]:
-        if t.shape != shape or t.stride() != stride or t.dtype != dtype or t.device != device:
-            raise ValueError("every layer must have the first layer's shape, strides, dtype and device")
-    sstride = s0.stride()
-    for s in scales:
-        if s.dtype != torch.float32 or s.shape != (pages, 2, hkv) or s.stride() != sstride or s.device != device:
-            raise ValueError(f"every layer's scales must be float32 [{pages}, 2, {hkv}] of the same strides on {device}")
+    if not _alike(layers, first):
+        raise ValueError("every layer must have the first layer's shape, strides, dtype and device")
+    if s0.dtype != torch.float32 or s0.shape != (pages, 2, hkv) or not _alike(scales, s0):
+        raise ValueError(f"every layer's scales must be float32 [{pages}, 2, {hkv}] of the same strides on {device}")
     return device, hkv, d, pages, page_size, (
-        _lib.ptr_array([t.data_ptr() for t in layers]), _lib.ptr_array([s.data_ptr() for s in scales]), len(layers),
-        CACHE_CODES[dtype], page_size, page_stride, v_offset, token_stride, head_stride, *sstride)
+        _pointers(layers), _pointers(scales), len(layers),
+        CACHE_CODES[first.dtype], page_size, page_stride, v_offset, token_stride, head_stride, *s0.stride())
 
 
 def append_quantized(
@@ -98,11 +116,9 @@ def append_quantized(
         raise TypeError(f"K/V rows must be float16 or bfloat16, got {first.dtype}")
     if first.ndim != 3 or tuple(first.shape[1:]) != (hkv, d) or not rows_contiguous(first):
         raise ValueError(f"K/V rows must be [nnz, {hkv}, {d}] with contiguous (Hkv, D), got {tuple(first.shape)}")
-    shape, stride, dtype = first.shape, first.stride(), first.dtype
-    for t in (*k_src, *v_src):
-        if t.shape != shape or t.dtype != dtype or t.device != device or t.stride() != stride:
-            raise ValueError("every K/V source must have the first one's shape, strides, dtype and device")
-    nnz = shape[0]
+    if first.device != device or not _alike(k_src, first) or not _alike(v_src, first):
+        raise ValueError(f"every K/V source must have the first one's shape, strides and dtype and be on {device}")
+    nnz, stride, dtype = first.shape[0], first.stride(), first.dtype
     batch = kv_last_page_len.numel()
     if batch == 0:
         raise ValueError("the batch must hold at least one request")
@@ -119,7 +135,7 @@ def append_quantized(
         raise ValueError("max_append must not be negative")
     with _lib.on_device(device):
         rc = _lib.load().atlas_kv_append_quantized(
-            *args, _lib.ptr_array([t.data_ptr() for t in k_src]), _lib.ptr_array([t.data_ptr() for t in v_src]),
+            *args, _pointers(k_src), _pointers(v_src),
             stride[0] if nnz > 1 else hkv * d, _lib.dtype_code(dtype), hkv, d, append_indptr.data_ptr(),
             kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), batch, int(max_append), nnz, pages,
             kv_indices.numel(), _lib.stream_of(device))
@@ -145,7 +161,7 @@ def commit_quantized(
 
     A destination block's scale becomes the largest of its own and those of the
     blocks its rows come from; when it grows, the block's other rows are rounded to
-    it.  At most 64 rows of one request; ``max_items`` is the most of any (read
+    it.  Of rows with one destination the last stays.  At most 64 rows of one request; ``max_items`` is the most of any (read
     back when left out), rows past it stay where they are.  Requests must not
     share the pages they write to."""
     device, hkv, d, pages, page_size, args = _check_layers(layers, scales, kv_layout, "commit_quantized")
