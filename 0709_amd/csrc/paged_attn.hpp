@@ -353,9 +353,9 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a, 
   const int rows = min(block_rows, r.q_len * a.group - row_start);
   const int lr = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (lr >= rows) return;
+  const int lane = threadIdx.x & 63;
   const Block k = plan_block(a, r, b, row_start, rows);
   if (k.splits <= 1) return;
-  const int lane = threadIdx.x & 63;
   const float* ws = static_cast<const float*>(p.workspace);
   const int64_t nrows = int64_t(p.batch) * p.num_kv_heads * p.row_blocks * p.num_splits * block_rows;
   const int64_t row0 = int64_t(item) * p.num_splits * block_rows + lr;

@@ -28,7 +28,6 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-#define SETPRIO(x) __builtin_amdgcn_s_setprio(x)
 template <int N>
 using Stage = std::integral_constant<int, N>;
 
@@ -81,10 +80,10 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int row_start = rb * p.block_rows;
   const int rows = min(p.block_rows, r.q_len * a.group - row_start);
   if (rows <= 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
   const Block k = plan_block(a, r, b, row_start, rows);
   if (split >= k.splits) return;
 
-  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r16 = lane & 15;
   const bool bf16 = p.dtype == ATLAS_DTYPE_BF16;
@@ -334,7 +333,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         }
       }
       __builtin_amdgcn_sched_barrier(0);
-      SETPRIO(1);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -345,7 +344,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = C::mfma(kf[kt][ks], qf[rt][ks], acc[rt][kt]);
-      SETPRIO(0);
+      __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
       frag vf[DT];  // V^T's operands by dim tile
 #pragma unroll
@@ -464,12 +463,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
           pf[rt][kt * 2 + 1] = C::pack(e[2], e[3]);
         }
       }
-      SETPRIO(1);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) o[rt][t] = C::mfma(vf[t], pf[rt], o[rt][t]);
-      SETPRIO(0);
+      __builtin_amdgcn_s_setprio(0);
       if (masked && strange) {
         // Where a row sees an infinity or NaN, its sum becomes one: a product with the
         // marks is zero for the rows that do not.

@@ -42,14 +42,16 @@ STREAM_ROWS_PAGES = 16
 WIDE_ROWS = 128
 # Requests of more packed rows than this take the kernel of many rows.
 MAX_STREAM_ROWS = 192
-# Workgroups to aim for when the keys are split, and the least keys of a split.
-# Decode splits are never longer than MAX_DECODE_SPLIT keys where the batch is
-# large: short splits even out requests of different lengths.
-DECODE_WORKGROUPS = 1024
-MAX_DECODE_SPLIT = 1536
-STREAM_WORKGROUPS = 512
-BLOCK_WORKGROUPS = 1024
+# Single tokens and few rows: splits as long as one per CU makes them, between these
+# (short splits even out requests of different lengths); a request of a single token whose
+# keys and values of a head are no more than WHOLE_BYTES is not split.
+CUS = 256
 MIN_SPLIT_KEYS = 256
+MAX_DECODE_SPLIT = 1536
+MAX_STREAM_SPLIT = 4096
+WHOLE_BYTES = 256 << 10
+# Many rows: the workgroups that run at once.
+BLOCK_WORKGROUPS = 512
 MAX_SPLITS = 256
 
 CACHE_CODES = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
@@ -59,33 +61,35 @@ _ARGS = struct.Struct("=14Q15q15i2f4x")
 
 
 def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int, *, tree: bool = False,
-                 quantized: bool = False, page_size: int = 16) -> tuple[bool, int, int, int, int]:
-    """(single token?, rows of a block, row blocks, splits, keys per split) of a call.
+                 row_bytes: int = 256, quantized: bool = False,
+                 page_size: int = 16) -> tuple[bool, int, int, int, int]:
+    """(single token?, rows of a block, row blocks, most splits, least keys of a split) of a
+    call.  ``row_bytes`` is a cache row's size.
 
     One query token per request takes blocks of 16 packed rows, more take equal
-    blocks.  Keys are split until about as many workgroups are there as the device
-    holds at once, in splits of at least MIN_SPLIT_KEYS; a request shorter than
-    ``max_kv_len`` takes fewer splits of the same size."""
+    blocks.  A request takes as many splits as its own length asks for."""
     single = max_q_len <= 1 and not tree
     rows = max(1, max_q_len * group)
     if single:
-        most_rows, target = DECODE_ROWS, DECODE_WORKGROUPS
+        most_rows = DECODE_ROWS
     elif rows <= MAX_STREAM_ROWS:
         most_rows = STREAM_ROWS_PAGES if page_size % 16 else (STREAM_ROWS_8BIT if quantized else STREAM_ROWS_16BIT)
-        target = STREAM_WORKGROUPS
     else:
-        most_rows, target = WIDE_ROWS, BLOCK_WORKGROUPS
+        most_rows = WIDE_ROWS
     blocks = -(-rows // most_rows)
     block_rows = 16 * -(-rows // (16 * blocks))
     items = batch * kv_heads * blocks
-    most = max(1, -(-max_kv_len // MIN_SPLIT_KEYS))
-    splits = min(most, target // items)
-    if single:
-        splits = max(splits, -(-max_kv_len // MAX_DECODE_SPLIT)) if max_kv_len > MAX_DECODE_SPLIT else 1
-    splits = max(1, min(MAX_SPLITS, splits))
-    keys = max(64, -(-max_kv_len // splits))
+    longest = max(1, max_kv_len)
+    if most_rows == WIDE_ROWS:
+        keys = max(MIN_SPLIT_KEYS, -(-longest // max(1, BLOCK_WORKGROUPS // items)))
+    elif single and 2 * row_bytes * longest <= WHOLE_BYTES:
+        keys = longest
+    else:
+        keys = max(MIN_SPLIT_KEYS, -(-longest // max(1, CUS // items)))
+        keys = min(keys, MAX_DECODE_SPLIT if single else MAX_STREAM_SPLIT)
+    keys = max(keys, -(-longest // MAX_SPLITS))
     keys = -(-keys // 64) * 64
-    return single, block_rows, blocks, max(1, -(-max_kv_len // keys)), keys
+    return single, block_rows, blocks, -(-longest // keys), keys
 
 
 def workspace_bytes(batch: int, kv_heads: int, head_dim: int, shape: tuple[bool, int, int, int, int]) -> int:
@@ -258,10 +262,11 @@ def paged_attention(
     if max_q_len < 0 or max_kv_len < 0:
         raise ValueError("max_q_len and max_kv_len must not be negative")
     max_q_len = min(int(max_q_len), nnz)
-    # (keys that a window leaves to a row block; the visible prefix comes on top)
-    reach = max_kv_len if window_left < 0 or prefix_lens is not None else min(max_kv_len, window_left + max_q_len)
+    # (keys that a window leaves to the rows; a visible prefix in front of it, which only the
+    # device knows, is taken to be short: a long one makes the splits longer)
+    reach = max_kv_len if window_left < 0 else min(max_kv_len, window_left + max_q_len)
     shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach), tree=mode == _lib.MASK_TREE,
-                         quantized=s is not None, page_size=page_size)
+                         row_bytes=d * base.element_size(), quantized=s is not None, page_size=page_size)
     need = workspace_bytes(batch, hkv, d, shape)
     if need:
         if workspace is None:
