@@ -28,8 +28,12 @@ The shared prefix is then read once per group instead of once per route.
 Routes that share nothing are planned one request each (qo_indptr =
 0, 1, ..., B), exactly like a prefill batch of single-query requests.
 
-Not supported (raise NotImplementedError): RoPE inside the kernel, sliding
-windows, logit soft-capping, and k_scale / v_scale other than 1.
+A plan with ``logits_soft_cap``, ``window_left``, ``pos_encoding_mode="ALIBI"`` or an
+8-bit ``kv_data_type`` runs on ``paged_attention.paged_attention`` instead
+(without the cascade); ``forward`` may then give each layer its own cap.
+
+Not supported (raise NotImplementedError): RoPE inside the kernel, and
+k_scale / v_scale other than 1 (an 8-bit cache has ``kv_block_scales``).
 """
 
 from __future__ import annotations
@@ -46,6 +50,7 @@ from .tree_attention import (
     MAX_ROWS_PER_ITEM,
     TILE_KEYS,
     BatchPrefillWithPagedKVCacheWrapper,
+    ScoredPlan,
     _dtype_from,
     _partial_row_bytes,
     _host_lists,
@@ -67,7 +72,7 @@ def _unit_scale(value, name: str) -> None:
             raise NotImplementedError(f"{name} must be a scalar")
         value = float(value.item())
     if float(value) != 1.0:
-        raise NotImplementedError(f"{name} other than 1 is not supported (fp16/bf16 KV only)")
+        raise NotImplementedError(f"{name} other than 1 is not supported (an 8-bit cache has kv_block_scales)")
 
 
 class BatchDecodeWithPagedKVCacheWrapper:
@@ -136,13 +141,11 @@ class BatchDecodeWithPagedKVCacheWrapper:
         disable_split_kv: bool = False,
         **_unused,
     ) -> None:
-        if pos_encoding_mode != "NONE":
-            raise NotImplementedError("only pos_encoding_mode='NONE' is supported (RoPE is applied by the caller)")
-        if window_left != -1 or logits_soft_cap not in (None, 0.0):
-            raise NotImplementedError("sliding windows and logit soft-capping are not supported")
         # FlashInfer: data_type is the older name of the KV (and q) type.
         q_dtype = _dtype_from(q_data_type if q_data_type is not None else data_type, torch.float16)
-        kv_dtype = _dtype_from(kv_data_type if kv_data_type is not None else data_type, q_dtype)
+        kv_dtype = _dtype_from(kv_data_type if kv_data_type is not None else data_type, q_dtype, codes=True)
+        scored = pos_encoding_mode != "NONE" or window_left != -1 or logits_soft_cap not in (None, 0.0) or \
+            kv_dtype in (torch.float8_e4m3fn, torch.int8)
         if isinstance(indptr, torch.Tensor):
             batch = int(indptr.numel()) - 1
         else:
@@ -151,7 +154,7 @@ class BatchDecodeWithPagedKVCacheWrapper:
             raise ValueError("indptr must describe at least one request")
         self._prefill.split_target_items = 1 if disable_split_kv else self.split_target_items
         self.cascade_groups = 0
-        if self.use_cascade and batch > 1 and not disable_split_kv:
+        if self.use_cascade and batch > 1 and not disable_split_kv and not scored:
             if self._plan_cascade(indptr, indices, last_page_len, int(num_qo_heads), int(num_kv_heads),
                                   int(head_dim), int(page_size), q_dtype, kv_dtype, sm_scale, non_blocking):
                 self._batch = batch
@@ -159,8 +162,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         qo = torch.arange(batch + 1, dtype=torch.int32)
         self._prefill.plan(
             qo, indptr, indices, last_page_len, num_qo_heads, num_kv_heads, head_dim, page_size,
-            causal=False, pos_encoding_mode="NONE", sm_scale=sm_scale, q_data_type=q_dtype, kv_data_type=kv_dtype,
-            non_blocking=non_blocking,
+            causal=window_left != -1, pos_encoding_mode=pos_encoding_mode, sm_scale=sm_scale, window_left=window_left,
+            logits_soft_cap=logits_soft_cap, q_data_type=q_dtype, kv_data_type=kv_dtype, non_blocking=non_blocking,
         )
         self._batch = batch
 
@@ -305,9 +308,11 @@ class BatchDecodeWithPagedKVCacheWrapper:
         out: torch.Tensor | None = None,
         lse: torch.Tensor | None = None,
         return_lse: bool = False,
+        kv_block_scales: torch.Tensor | None = None,
         **_unused,
     ):
-        """q: [batch, Hq, D] -> out [batch, Hq, D] (and lse [batch, Hq])."""
+        """q: [batch, Hq, D] -> out [batch, Hq, D] (and lse [batch, Hq]), over an
+        8-bit cache with its ``kv_block_scales`` [pages, 2, Hkv]."""
         if self._batch == 0:
             raise RuntimeError("plan() must be called before run()")
         _unit_scale(q_scale, "q_scale")
@@ -315,7 +320,8 @@ class BatchDecodeWithPagedKVCacheWrapper:
         _unit_scale(v_scale, "v_scale")
         if q.ndim != 3 or int(q.shape[0]) != self._batch:
             raise ValueError(f"q must be [{self._batch}, Hq, D] (one query per planned request), got {tuple(q.shape)}")
-        return self._prefill.run(q, paged_kv_cache, out=out, lse=lse, return_lse=return_lse)
+        return self._prefill.run(q, paged_kv_cache, out=out, lse=lse, return_lse=return_lse,
+                                 kv_block_scales=kv_block_scales)
 
     def forward(
         self,
@@ -330,20 +336,35 @@ class BatchDecodeWithPagedKVCacheWrapper:
         sm_scale: float | None = None,
         rope_scale: float | None = None,
         rope_theta: float | None = None,
+        kv_block_scales: torch.Tensor | None = None,
     ) -> torch.Tensor:
-        """The older entry point SGLang calls; sm_scale here overrides the plan's."""
-        if pos_encoding_mode != "NONE":
-            raise NotImplementedError("only pos_encoding_mode='NONE' is supported (RoPE is applied by the caller)")
-        if window_left != -1 or logits_soft_cap not in (None, 0.0):
-            raise NotImplementedError("sliding windows and logit soft-capping are not supported")
+        """The older entry point SGLang calls; sm_scale here overrides the plan's,
+        and so does logits_soft_cap where the plan is of scored attention."""
         plan = self._prefill.current_plan
         if plan is None:
             raise RuntimeError("plan() must be called before forward()")
+        scored = isinstance(plan, ScoredPlan)
+        if pos_encoding_mode != "NONE" and not (pos_encoding_mode == "ALIBI" and scored and
+                                                plan.alibi_slopes is not None):
+            raise NotImplementedError(f"pos_encoding_mode={pos_encoding_mode!r} is not the plan's "
+                                      "(RoPE is applied by the caller)")
+        if window_left != -1 and not (scored and window_left == plan.window_left):
+            raise NotImplementedError("plan with the sliding window")
+        changes = {}
+        if logits_soft_cap is not None and float(logits_soft_cap) != (plan.soft_cap if scored else 0.0):
+            if not scored:
+                raise NotImplementedError("plan with a logits_soft_cap, or with another option of scored attention")
+            if not 0.0 <= float(logits_soft_cap) < math.inf:
+                raise ValueError("logits_soft_cap must be finite and not negative")
+            changes["soft_cap"] = float(logits_soft_cap)
         if sm_scale is not None:
+            changes["sm_scale"] = float(sm_scale)
+        if changes:
             # a copy: a later plan() of the same shape may hand back the
             # cached plan object, which keeps the plan's own scale
-            self._prefill._plan = dataclasses.replace(plan, sm_scale=float(sm_scale))
-        return self.run(q, paged_kv_cache, q_scale=q_scale, k_scale=k_scale, v_scale=v_scale)
+            self._prefill._plan = dataclasses.replace(plan, **changes)
+        return self.run(q, paged_kv_cache, q_scale=q_scale, k_scale=k_scale, v_scale=v_scale,
+                        kv_block_scales=kv_block_scales)
 
     def end_forward(self) -> None:
         """FlashInfer keeps this as a no-op."""

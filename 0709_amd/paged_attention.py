@@ -61,13 +61,17 @@ _ARGS = struct.Struct("=14Q15q15i2f4x")
 
 
 def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_len: int, *, tree: bool = False,
-                 row_bytes: int = 256, quantized: bool = False,
+                 window_left: int = -1, row_bytes: int = 256, quantized: bool = False,
                  page_size: int = 16) -> tuple[bool, int, int, int, int]:
     """(single token?, rows of a block, row blocks, most splits, least keys of a split) of a
     call.  ``row_bytes`` is a cache row's size.
 
     One query token per request takes blocks of 16 packed rows, more take equal
-    blocks.  A request takes as many splits as its own length asks for."""
+    blocks.  A request takes as many splits as its own length asks for.  Behind a window
+    the splits are sized for its keys; a visible prefix in front of it, which only the
+    device knows, is taken to be short (a long one makes the splits longer)."""
+    if window_left >= 0:
+        max_kv_len = min(max_kv_len, window_left + max_q_len)
     single = max_q_len <= 1 and not tree
     rows = max(1, max_q_len * group)
     if single:
@@ -262,11 +266,8 @@ def paged_attention(
     if max_q_len < 0 or max_kv_len < 0:
         raise ValueError("max_q_len and max_kv_len must not be negative")
     max_q_len = min(int(max_q_len), nnz)
-    # (keys that a window leaves to the rows; a visible prefix in front of it, which only the
-    # device knows, is taken to be short: a long one makes the splits longer)
-    reach = max_kv_len if window_left < 0 else min(max_kv_len, window_left + max_q_len)
-    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(reach), tree=mode == _lib.MASK_TREE,
-                         row_bytes=d * base.element_size(), quantized=s is not None, page_size=page_size)
+    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(max_kv_len), tree=mode == _lib.MASK_TREE,
+                         window_left=window_left, row_bytes=d * base.element_size(), quantized=s is not None, page_size=page_size)
     need = workspace_bytes(batch, hkv, d, shape)
     if need:
         if workspace is None:

@@ -78,6 +78,36 @@ class AttentionPlan:
         return int(self.meta.data_ptr()) + 4 * offset
 
 
+@dataclass
+class ScoredPlan:
+    """A plan for ``paged_attention``: device metadata, masks and score options."""
+
+    batch: int
+    num_qo_heads: int
+    num_kv_heads: int
+    head_dim: int
+    page_size: int
+    sm_scale: float
+    q_dtype: torch.dtype
+    kv_dtype: torch.dtype
+    nnz: int
+    mask_mode: int
+    qo_indptr: torch.Tensor
+    kv_indptr: torch.Tensor
+    kv_last_page_len: torch.Tensor
+    kv_indices: torch.Tensor
+    tree_mask: torch.Tensor | None
+    mask_col_start: torch.Tensor
+    mask_words: int
+    kv_lens: list[int]
+    qo_lens: list[int]
+    window_left: int
+    soft_cap: float
+    alibi_slopes: torch.Tensor | None
+    workspace: torch.Tensor | None  # for the split states, None: torch's allocator
+    fused_append: bool = False
+
+
 def tensor_version(t: torch.Tensor) -> int | None:
     """The tensor's in-place version counter, or None for an inference tensor
     (created under torch.inference_mode, which keeps no counter)."""
@@ -127,13 +157,16 @@ def _host_lists(*items: torch.Tensor | list | tuple) -> list[list[int]]:
     return out  # type: ignore[return-value]
 
 
-def _dtype_from(value, default: torch.dtype) -> torch.dtype:
+def _dtype_from(value, default: torch.dtype, codes: bool = False) -> torch.dtype:
+    """The dtype of a name or dtype; ``codes``: an 8-bit cache's too."""
     if value is None:
         return default
     if isinstance(value, torch.dtype):
         return value
     name = str(value).replace("torch.", "")
     table = {"float16": torch.float16, "half": torch.float16, "bfloat16": torch.bfloat16}
+    if codes:
+        table.update(float8_e4m3fn=torch.float8_e4m3fn, int8=torch.int8)
     if name not in table:
         raise TypeError(f"unsupported data type {value!r}")
     return table[name]
@@ -276,6 +309,13 @@ class BatchPrefillWithPagedKVCacheWrapper:
     ``float_workspace_buffer`` holds the split-KV partial states (like
     FlashInfer's workspace: the partial O in the output dtype and an fp32 LSE
     per row); its size bounds how finely keys are split.
+
+    A plan with ``logits_soft_cap``, ``window_left`` (with ``causal=True``),
+    ``pos_encoding_mode="ALIBI"`` (the usual slopes of ``num_qo_heads``) or an
+    8-bit ``kv_data_type`` (float8_e4m3fn, int8; ``run`` then takes the cache's
+    ``kv_block_scales``) runs on ``paged_attention.paged_attention``, whose splits are
+    computed on the device; it takes the split states from torch's allocator
+    where the workspace is too small for them, and has no fused append.
     """
 
     def __init__(
@@ -308,6 +348,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         self._meta_buf: torch.Tensor | None = None
         self._indices_buf: torch.Tensor | None = None
         self._bits_buf: torch.Tensor | None = None
+        self._alibi: tuple[int, torch.Tensor] | None = None
 
     @property
     def device(self) -> torch.device:
@@ -341,12 +382,20 @@ class BatchPrefillWithPagedKVCacheWrapper:
     ) -> None:
         device = self.device
         _lib.require_device(self._workspace, what="BatchPrefillWithPagedKVCacheWrapper")
-        if pos_encoding_mode != "NONE":
-            raise NotImplementedError("only pos_encoding_mode='NONE' is supported (RoPE is applied by the caller)")
+        if pos_encoding_mode not in ("NONE", "ALIBI"):
+            raise NotImplementedError(
+                "only pos_encoding_mode 'NONE' and 'ALIBI' are supported (RoPE is applied by the caller)")
         if head_dim_vo is not None and int(head_dim_vo) != int(head_dim_qk):
             raise NotImplementedError("head_dim_vo must equal head_dim_qk")
-        if window_left != -1 or logits_soft_cap not in (None, 0.0):
-            raise NotImplementedError("sliding windows and logit soft-capping are not supported")
+        window_left, cap = int(window_left), float(logits_soft_cap or 0.0)
+        alibi = pos_encoding_mode == "ALIBI"
+        masked = custom_mask is not None or packed_custom_mask is not None
+        if window_left < -1 or not 0.0 <= cap < math.inf:
+            raise ValueError("window_left must be -1 (none) or not negative, logits_soft_cap finite and not negative")
+        if window_left >= 0 and not causal:
+            raise NotImplementedError("sliding windows need causal=True")
+        if alibi and masked:
+            raise NotImplementedError("a distance bias does not go with a custom mask (its nodes stand in no order)")
         hq, hkv, d, ps = int(num_qo_heads), int(num_kv_heads), int(head_dim_qk), int(page_size)
         if hq <= 0 or hkv <= 0 or hq % hkv != 0:
             raise ValueError("num_qo_heads must be a positive multiple of num_kv_heads")
@@ -355,9 +404,12 @@ class BatchPrefillWithPagedKVCacheWrapper:
         if ps <= 0:
             raise ValueError("page_size must be positive")
         q_dtype = _dtype_from(q_data_type, torch.float16)
-        kv_dtype = _dtype_from(kv_data_type, q_dtype)
-        if q_dtype != kv_dtype:
-            raise NotImplementedError("q and kv data types must match")
+        kv_dtype = _dtype_from(kv_data_type, q_dtype, codes=True)
+        codes = kv_dtype in (torch.float8_e4m3fn, torch.int8)
+        if q_dtype != kv_dtype and not codes:
+            raise NotImplementedError("q and kv data types must match, or the cache hold float8_e4m3fn or int8")
+        if codes and q_dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"q must be float16 or bfloat16 over an 8-bit cache, not {q_dtype}")
 
         qo, kvp, last = _host_lists(qo_indptr, paged_kv_indptr, paged_kv_last_page_len)
         batch = len(qo) - 1
@@ -436,6 +488,14 @@ class BatchPrefillWithPagedKVCacheWrapper:
                     mask_words = max(2, max(int(t.shape[1]) for t in tiles))
                     tree_bits = torch.cat([torch.nn.functional.pad(t, (0, mask_words - int(t.shape[1])))
                                            for t in tiles]).reshape(-1)
+
+        if codes or alibi or window_left >= 0 or cap > 0.0:
+            self._install_scored(
+                batch=batch, hq=hq, hkv=hkv, d=d, ps=ps, sm_scale=sm_scale, q_dtype=q_dtype, kv_dtype=kv_dtype,
+                mask_mode=mask_mode, qo=qo, kvp=kvp, last=last, cols=cols, kv_lens=kv_lens, qo_lens=qo_lens,
+                indices_src=paged_kv_indices.reshape(-1), tree_bits=tree_bits, mask_words=mask_words,
+                window_left=window_left, soft_cap=cap, alibi=alibi)
+            return
 
         # ---- work decomposition (the same inputs give the same work list) ----
         ws_rows_cap = self._workspace.numel() * self._workspace.element_size() // _partial_row_bytes(d)
@@ -620,6 +680,82 @@ class BatchPrefillWithPagedKVCacheWrapper:
         )
         self._plan_cache = (plan_key, self._plan)
 
+    def _install_scored(self, *, batch, hq, hkv, d, ps, sm_scale, q_dtype, kv_dtype, mask_mode, qo, kvp, last, cols,
+                        kv_lens, qo_lens, indices_src, tree_bits, mask_words, window_left, soft_cap, alibi) -> None:
+        """Make a plan for ``paged_attention`` the current one: the batch's metadata in
+        buffers that keep their addresses across plans that fit them, so a graph
+        captured over run() is right after a re-plan of the same batch size and
+        no more query rows per request whose page table fits too (1024 entries, or the
+        largest table planned before the capture); longer requests than at the
+        capture run in the splits of then."""
+        from .paged_attention import default_alibi_slopes, launch_shape, workspace_bytes
+
+        if qo[0] != 0:
+            raise ValueError("qo_indptr must start at 0")
+        device = self.device
+        meta_np = np.asarray((*qo, *kvp, *last, *cols), dtype=np.int32)
+        meta = self._persistent("_scored_meta_buf", len(meta_np), torch.int32)
+        _lib.staging().upload(meta_np, device, out=meta[: len(meta_np)])
+        n_idx = int(indices_src.numel())
+        indices = self._persistent("_scored_indices_buf", n_idx, torch.int32)
+        indices[:n_idx].copy_(indices_src)
+        if int(indices.numel()) * ps >= 1 << 31:
+            indices = indices[:n_idx]
+        words = None
+        if tree_bits is not None:
+            words = self._persistent("_scored_bits_buf", int(tree_bits.numel()), torch.int64)[: int(tree_bits.numel())]
+            words.copy_(tree_bits.reshape(-1))
+            words = words.view(-1, mask_words)
+        slopes = None
+        if alibi:
+            if self._alibi is None or self._alibi[0] != hq:
+                self._alibi = (hq, default_alibi_slopes(hq, device))
+            slopes = self._alibi[1]
+        shape = launch_shape(
+            batch, hkv, hq // hkv, max(qo_lens), max(kv_lens), tree=words is not None, window_left=window_left,
+            row_bytes=d * kv_dtype.itemsize, quantized=kv_dtype != q_dtype, page_size=ps)
+        ws = self._workspace
+        if ws.numel() * ws.element_size() < workspace_bytes(batch, hkv, d, shape) or ws.data_ptr() % 16:
+            ws = None
+        part = np.cumsum((0, batch + 1, batch + 1, batch, batch)).tolist()
+        self._plan = ScoredPlan(
+            batch=batch, num_qo_heads=hq, num_kv_heads=hkv, head_dim=d, page_size=ps,
+            sm_scale=float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d), q_dtype=q_dtype,
+            kv_dtype=kv_dtype, nnz=qo[-1] - qo[0], mask_mode=mask_mode, qo_indptr=meta[part[0]: part[1]],
+            kv_indptr=meta[part[1]: part[2]], kv_last_page_len=meta[part[2]: part[3]],
+            mask_col_start=meta[part[3]: part[4]], kv_indices=indices, tree_mask=words, mask_words=mask_words,
+            kv_lens=kv_lens, qo_lens=qo_lens, window_left=window_left, soft_cap=soft_cap, alibi_slopes=slopes,
+            workspace=ws)
+
+    def _run_scored(self, plan, q, paged_kv_cache, *, kv_block_scales, out, lse, return_lse):
+        from .paged_attention import paged_attention
+
+        base = paged_kv_cache[0] if isinstance(paged_kv_cache, (tuple, list)) else paged_kv_cache
+        td, hd = (-2, -3) if self._kv_layout == "HND" else (-3, -2)
+        if base.ndim < 4 or (base.shape[td], base.shape[hd], base.shape[-1]) != \
+                (plan.page_size, plan.num_kv_heads, plan.head_dim):
+            raise ValueError(f"kv cache {tuple(base.shape)} does not match the plan's (page_size, Hkv, D) "
+                             f"({plan.page_size}, {plan.num_kv_heads}, {plan.head_dim})")
+        if q.dtype != plan.q_dtype or base.dtype != plan.kv_dtype:
+            raise TypeError(f"dtype mismatch: q {q.dtype}, kv {base.dtype}, planned {plan.q_dtype}, {plan.kv_dtype}")
+        if q.ndim != 3 or tuple(q.shape[1:]) != (plan.num_qo_heads, plan.head_dim) or int(q.shape[0]) < plan.nnz:
+            raise ValueError(f"q must be [nnz, {plan.num_qo_heads}, {plan.head_dim}], got {tuple(q.shape)}")
+        want_lse = return_lse or lse is not None
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if want_lse and lse is None:
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        # (the plan's rows: q may be padded)
+        paged_attention(
+            q[: plan.nnz], paged_kv_cache, plan.qo_indptr, plan.kv_indptr, plan.kv_indices, plan.kv_last_page_len,
+            max_q_len=max(plan.qo_lens), max_kv_len=max(plan.kv_lens), kv_block_scales=kv_block_scales,
+            causal=plan.mask_mode == _lib.MASK_CAUSAL, tree_mask=plan.tree_mask,
+            mask_col_start=plan.mask_col_start if plan.tree_mask is not None else None, window_left=plan.window_left,
+            logits_soft_cap=plan.soft_cap, alibi_slopes=plan.alibi_slopes, sm_scale=plan.sm_scale,
+            kv_layout=self._kv_layout, out=out[: plan.nnz], lse=lse[: plan.nnz] if want_lse else None,
+            workspace=plan.workspace)
+        return (out, lse) if want_lse else out
+
     @property
     def kv_layout(self) -> str:
         """The paged layout run() reads: "NHD" or "HND"."""
@@ -658,8 +794,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
         append_key_states: torch.Tensor | None = None,
         append_value_states: torch.Tensor | None = None,
         rope_cos_sin: tuple[torch.Tensor, torch.Tensor] | None = None,
+        kv_block_scales: torch.Tensor | None = None,
     ):
-        """Attention of the planned batch.  With ``append_key_states`` and
+        """Attention of the planned batch, over an 8-bit cache with its
+        ``kv_block_scales`` [pages, 2, Hkv].  With ``append_key_states`` and
         ``append_value_states`` ([nnz, Hkv, D], one row per query token), each
         request's rows are first written to its last qo_len key positions,
         inside the same launch: ``write_suffix_kv`` followed by ``run`` as one
@@ -677,6 +815,13 @@ class BatchPrefillWithPagedKVCacheWrapper:
         plan = self._plan
         if plan is None:
             raise RuntimeError("plan() must be called before run()")
+        if isinstance(plan, ScoredPlan):
+            if append_key_states is not None or append_value_states is not None or rope_cos_sin is not None:
+                raise NotImplementedError("a plan with scored attention or an 8-bit cache has no fused append")
+            return self._run_scored(plan, q, paged_kv_cache, kv_block_scales=kv_block_scales, out=out, lse=lse,
+                                    return_lse=return_lse)
+        if kv_block_scales is not None:
+            raise ValueError("kv_block_scales goes with a plan of an 8-bit kv_data_type")
         hnd = self._kv_layout == "HND"
         # (token, head) dims of a page: NHD pages [.., page_size, Hkv, D],
         # HND pages [.., Hkv, page_size, D]
