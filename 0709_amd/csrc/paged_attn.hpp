@@ -289,24 +289,17 @@ __device__ __forceinline__ int slot_of(const PagedAttnArgs& a, int key) {
   return int((uint64_t(uint32_t(key)) * a.page_magic) >> a.page_bits);
 }
 
-// Pages of the 16-key tiles of one step, for page sizes that are multiples of 16.
-// Lane l holds what belongs to tile l % KT: its page id, read steps before the step's
-// rows are asked for; one step later the offset of the tile's first row and the
-// page's scales (K's in lanes of even l / KT, V's in the others).  The tiles' values come
-// back by readlane, and no memory access of the key loop waits for another.
-template <bool Q8, int KT>
-struct TilePages {
-  const int32_t* ids;  // the request's page ids
-  const float* scales;
-  int64_t scale_page, page_stride;
+// A request's page ids.  For page sizes that are multiples of 16 the kernels read
+// what a run of 16-key tiles needs by lane, once for many steps, and take a tile's by
+// readlane: no memory access of the key loop waits for another.
+struct Pages {
+  const int32_t* ids;
+  int64_t page_stride;
   int64_t last_id;  // ids are clamped to [0, last_id]
   int page_size, ts;
 
-  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const Request& r, int h, int lane) {
+  __device__ __forceinline__ void begin(const PagedAttnArgs& a, const Request& r) {
     ids = a.p.kv_indices + r.pt;
-    if constexpr (Q8)
-      scales = a.p.kv_scales + int64_t(h) * a.p.scale_stride_head + ((lane / KT) & 1) * a.p.scale_stride_kv;
-    scale_page = a.p.scale_stride_page;
     page_stride = a.p.page_stride;
     last_id = a.p.num_pages - 1;
     page_size = a.p.page_size;
@@ -325,17 +318,10 @@ struct TilePages {
   __device__ __forceinline__ int64_t row_offset(const PagedAttnArgs& a, int id, int tile) const {
     return valid(id) * page_stride + int64_t((tile - slot_of(a, tile) * page_size) * ts);
   }
-  __device__ __forceinline__ float read_scale(int id) const {
-    if constexpr (Q8) return scales[valid(id) * scale_page];
-    else return 0.f;
-  }
   static __device__ __forceinline__ int64_t tile_row(int64_t v, int kt) {
     const uint32_t lo = __builtin_amdgcn_readlane(uint32_t(v), kt);
     const uint32_t hi = __builtin_amdgcn_readlane(uint32_t(uint64_t(v) >> 32), kt);
     return int64_t((uint64_t(hi) << 32) | lo);
-  }
-  static __device__ __forceinline__ float tile_scale(float v, int kv, int kt) {
-    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), kv * KT + kt));
   }
 };
 

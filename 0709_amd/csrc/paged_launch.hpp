@@ -7,22 +7,35 @@
 namespace atlas {
 namespace {
 
+// Few rows stream: as many row tiles as the registers hold beside a step's K and V (page
+// sizes that look every key up: one; 16-bit rows: two; codes: three).
 template <int KIND, int D, bool PAGE16, bool SCORED>
 void launch_paged_kernel(const PagedAttnArgs& a, hipStream_t stream) {
   const atlas_paged_attn_t& p = a.p;
   const int64_t units = int64_t(p.batch) * p.num_kv_heads * p.num_splits;
-  const dim3 grid(static_cast<unsigned>(p.row_blocks == 1 ? units : (units + 7) / 8 * 8 * p.row_blocks)), block(kPaThreads);
-  if (p.single_token)
+  const dim3 grid(static_cast<unsigned>(p.row_blocks == 1 ? units : (units + 7) / 8 * 8 * p.row_blocks));
+  const dim3 block(kPaThreads);
+  if (p.single_token) {
     hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 1, PAGE16, SCORED, false>), grid, block, 0, stream, a);
-  else if (p.block_rows <= 16)
+    return;
+  }
+  if (p.block_rows <= 16) {
     hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 1, PAGE16, SCORED, true>), grid, block, 0, stream, a);
-  else if (PAGE16 && p.block_rows <= 32)
-    hipLaunchKernelGGL((paged_stream_kernel<KIND, D, PAGE16 ? 2 : 1, PAGE16, SCORED, true>), grid, block, 0, stream, a);
-  else if (PAGE16 && Cache<KIND>::kQuant && p.block_rows <= 48)
-    hipLaunchKernelGGL((paged_stream_kernel<KIND, D, PAGE16 && Cache<KIND>::kQuant ? 3 : 1, PAGE16, SCORED, true>), grid,
-                       block, 0, stream, a);
-  else
-    hipLaunchKernelGGL((paged_rows_kernel<KIND, D, 2, PAGE16, SCORED>), grid, block, 0, stream, a);
+    return;
+  }
+  if constexpr (PAGE16) {
+    if (p.block_rows <= 32) {
+      hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 2, PAGE16, SCORED, true>), grid, block, 0, stream, a);
+      return;
+    }
+    if constexpr (Cache<KIND>::kQuant) {
+      if (p.block_rows <= 48) {
+        hipLaunchKernelGGL((paged_stream_kernel<KIND, D, 3, PAGE16, SCORED, true>), grid, block, 0, stream, a);
+        return;
+      }
+    }
+  }
+  hipLaunchKernelGGL((paged_rows_kernel<KIND, D, PAGE16, SCORED>), grid, block, 0, stream, a);
 }
 
 template <int KIND, int D>

@@ -1,10 +1,10 @@
 // Paged attention for many packed rows: prompts' chunks and wide draft trees.
 //
-// A workgroup of four waves takes up to 64 * RT packed rows of one KV head and one
-// split of the request's keys.  Tiles of 64 keys go from HBM through registers into
-// LDS as 16-bit rows (8-bit codes are converted on the way, once for all rows), one
-// tile ahead of the products, in two stages: the tile's loads are in flight while the
-// one before it is computed.  Row tiles of 16 go round the waves; K's operand is a
+// A workgroup of four waves takes up to 128 packed rows of one KV head and one split
+// of the request's keys.  Tiles of 32 keys (64 at head_dim 64) go from HBM through
+// registers into LDS as 16-bit rows (8-bit codes are converted on the way, once for all
+// rows): one tile is computed from one of two stages, the next is written to the
+// other, and two more are on their way.  Row tiles of 16 go round the waves; K's operand is a
 // 16-byte LDS read, V's two transposing reads.  A row's 16-byte granules are swapped
 // by the key so that neither the writes nor either kind of read meets in a bank.
 #pragma once
@@ -31,15 +31,15 @@ __device__ __forceinline__ void lds_barrier() {
 template <int N>
 using Stage = std::integral_constant<int, N>;
 
-// KIND: what the cache holds.  D: head_dim.  RT: row tiles of a wave.  PAGE16: page_size
-// is a multiple of 16, so a 16-key tile lies in one page and its id and scales are
+// KIND: what the cache holds.  D: head_dim.  PAGE16: page_size is a multiple of 16, so a 16-key tile lies in one page and its id and scales are
 // wave-uniform; other page sizes look every key up.  SCORED: scores may be capped or
 // biased, or their factor negative.
-template <int KIND, int D, int RT, bool PAGE16, bool SCORED>
+template <int KIND, int D, bool PAGE16, bool SCORED>
 __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs a) {
   typedef Cache<KIND> C;
   typedef typename C::frag frag;
   constexpr bool Q8 = C::kQuant;
+  constexpr int RT = 2;                    // row tiles of a wave
   constexpr int TK = D == 128 ? 32 : 64;  // keys of a tile
   constexpr int SUB = kChunk / TK;         // tiles of a chunk
   constexpr int NT = TK / 16;              // its 16-key tiles
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const char* vbase = kbase + p.v_offset;
   const int ts = int(p.token_stride);
   const int page_size = p.page_size;
-  TilePages<Q8, NT> pages;
-  pages.begin(a, r, h, lane);
+  Pages pages;
+  pages.begin(a, r);
 
   auto key_of = [&](int c) __attribute__((always_inline)) {
     return (c < k.ca * SUB ? c : c - k.ca * SUB + k.cb * SUB) * TK;
@@ -144,7 +144,6 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     lo = c < k.ca * SUB ? 0 : k.lo;
     hi = (c < k.ca * SUB ? k.prefix : k.hi) - 1;
   };
-  typedef TilePages<Q8, NT> Tiles;
   // 64 / NT tiles make a window: lane l holds the offset of the first row of 16-key tile
   // l % NT of its tile l / NT, and that page's scales.  A window is read at once, when
   // its first tile is asked for, so that the loads of the key loop are all alike and
@@ -159,7 +158,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     const int mine = min(c + lane / NT, win1 - 1);
     int lo, hi;
     bounds(mine, lo, hi);
-    const int tile = Tiles::tile_key(key_of(mine), lane & (NT - 1), lo, hi);
+    const int tile = Pages::tile_key(key_of(mine), lane & (NT - 1), lo, hi);
     const int id = pages.read_id(a, tile);
     win_rows = pages.row_offset(a, id, tile);
     if constexpr (Q8) {
@@ -190,11 +189,11 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       if constexpr (PAGE16) {
         // (a wave's rows of one piece lie in one 16-key tile)
         const int kt = (j * RSTEP + wave * (64 / GG)) >> 4;
-        const int64_t row0 = Tiles::tile_row(win_rows, (c - win0) * NT + kt);
+        const int64_t row0 = Pages::tile_row(win_rows, (c - win0) * NT + kt);
         uint32_t off = piece_at;
         if (!whole) {
           const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
-          off = uint32_t((key - Tiles::tile_key(kb, kt, lo, hi)) * ts + piece * 16);
+          off = uint32_t((key - Pages::tile_key(kb, kt, lo, hi)) * ts + piece * 16);
         }
         x.k[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
         x.v[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);

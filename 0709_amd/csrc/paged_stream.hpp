@@ -17,15 +17,15 @@
 namespace atlas {
 namespace {
 
-template <int NB>
+template <int BYTES>
 __device__ __forceinline__ void load_words(const char* p, uint32_t* out) {
-  if constexpr (NB == 16) {
+  if constexpr (BYTES == 16) {
     const w4 v = __builtin_nontemporal_load(reinterpret_cast<const w4*>(p));
     out[0] = v[0];
     out[1] = v[1];
     out[2] = v[2];
     out[3] = v[3];
-  } else if constexpr (NB == 8) {
+  } else if constexpr (BYTES == 8) {
     const w2 v = __builtin_nontemporal_load(reinterpret_cast<const w2*>(p));
     out[0] = v[0];
     out[1] = v[1];
@@ -54,7 +54,6 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   constexpr int VW = VB / 4;
   constexpr int OS = D + 4;               // LDS row stride (floats)
   constexpr int NS = PAGE16 ? KT : KT * 4;  // scales of a step: by tile or by key
-  constexpr int NB = RT > 1 ? 1 : 2;      // steps in registers
   constexpr bool QLDS = RT > 1;           // more than one tile of queries stays in LDS
   const atlas_paged_attn_t& p = a.p;
 
@@ -158,8 +157,8 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   const char* vbase = kbase + p.v_offset;
   const int ts = int(p.token_stride);
   const int page_size = p.page_size;
-  TilePages<Q8, KT> pages;
-  pages.begin(a, r, h, lane);
+  Pages pages;
+  pages.begin(a, r);
 
   struct RawK {
     uint32_t k[KT][KL * 4];
@@ -181,7 +180,6 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   // Up to 64 / KT steps make a window: lane l holds the offset of the first row of
   // tile l % KT of its step l / KT, and that page's scales, read together before the
   // window's first step.
-  typedef TilePages<Q8, KT> Tiles;
   constexpr int WIN = 64 / KT;
   int64_t win_rows = 0;
   float win_ks = 0.f, win_vs = 0.f;
@@ -191,7 +189,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
     const int mine = min(s + lane / KT, end - 1);
     int lo, hi;
     bounds(mine, lo, hi);
-    const int tile = Tiles::tile_key(key_of(mine), lane & (KT - 1), lo, hi);
+    const int tile = Pages::tile_key(key_of(mine), lane & (KT - 1), lo, hi);
     const int id = pages.read_id(a, tile);
     win_rows = pages.row_offset(a, id, tile);
     if constexpr (Q8) {
@@ -213,9 +211,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
     for (int kt = 0; kt < KT; ++kt) {
       const int t0 = kb + kt * 16;
       if constexpr (PAGE16) {
-        const char* kp = kbase + Tiles::tile_row(win_rows, (s - win0) * KT + kt);
+        const char* kp = kbase + Pages::tile_row(win_rows, (s - win0) * KT + kt);
         uint32_t ko = k_lane;
-        if (!whole) ko = uint32_t((min(max(t0 + r16, lo), hi) - Tiles::tile_key(kb, kt, lo, hi)) * ts + g * 16);
+        if (!whole) ko = uint32_t((min(max(t0 + r16, lo), hi) - Pages::tile_key(kb, kt, lo, hi)) * ts + g * 16);
 #pragma unroll
         for (int j = 0; j < KL; ++j) load_words<16>(kp + (ko + j * 64), &x.k[kt][4 * j]);
         if constexpr (Q8) {
@@ -249,12 +247,12 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
     for (int kt = 0; kt < KT; ++kt) {
       const int t0 = kb + kt * 16;
       if constexpr (PAGE16) {
-        const char* vp = vbase + Tiles::tile_row(win_rows, (s - win0) * KT + kt);
+        const char* vp = vbase + Pages::tile_row(win_rows, (s - win0) * KT + kt);
         uint32_t vo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) vo[i] = v_lane + uint32_t(i * ts);
         if (!whole) {
-          const int tile = Tiles::tile_key(kb, kt, lo, hi);
+          const int tile = Pages::tile_key(kb, kt, lo, hi);
 #pragma unroll
           for (int i = 0; i < 4; ++i) vo[i] = uint32_t((min(max(t0 + 4 * g + i, lo), hi) - tile) * ts + r16 * VB);
         }
@@ -450,19 +448,16 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
     const int end = PAGE16 ? min(s1, s + WIN) : s1;
     if constexpr (PAGE16) open_window(s, end);
     auto at = [&](int t) { return min(t, end - 1); };
-    if constexpr (NB > 1) {
-      // NB - 1 steps are in flight while one is computed; past the window's last step it
+    if constexpr (RT == 1) {
+      // One step is in flight while another is computed; past the window's last step it
       // is asked for again rather than branched around, so the waits stay exact.
-      RawK xk[NB];
-      RawV xv[NB];
-#pragma unroll
-      for (int i = 0; i < NB - 1; ++i) {
-        load_k(xk[i], at(s + i));
-        load_v(xv[i], at(s + i));
-      }
-      auto step = [&](int cur, int last) __attribute__((always_inline)) {
-        load_k(xk[last], at(s + NB - 1));
-        load_v(xv[last], at(s + NB - 1));
+      RawK xk[2];
+      RawV xv[2];
+      load_k(xk[0], s);
+      load_v(xv[0], s);
+      auto step = [&](int cur) __attribute__((always_inline)) {
+        load_k(xk[1 - cur], at(s + 1));
+        load_v(xv[1 - cur], at(s + 1));
         scores(xk[cur]);
         if (masked_step(s)) {
           weights(std::true_type{}, s, xk[cur].ks, xk[cur].vs);
@@ -473,12 +468,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
         }
         return ++s < end;
       };
-      if constexpr (NB == 2) {
-        while (step(0, 1) && step(1, 0)) {
-        }
-      } else {
-        while (step(0, 2) && step(1, 0) && step(2, 1)) {
-        }
+      while (step(0) && step(1)) {
       }
     } else {
       // The rows of O leave room for one step: the next step's K is asked for when the

@@ -265,6 +265,8 @@ def paged_attention(
             max_kv_len = max((b - a - 1) * page_size + n if b > a else 0 for a, b, n in zip(kvp, kvp[1:], last))
     if max_q_len < 0 or max_kv_len < 0:
         raise ValueError("max_q_len and max_kv_len must not be negative")
+    if max_q_len == 0:
+        return (out, lse) if return_lse else out
     max_q_len = min(int(max_q_len), nnz)
     shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(max_kv_len), tree=mode == _lib.MASK_TREE,
                          window_left=window_left, row_bytes=d * base.element_size(), quantized=s is not None, page_size=page_size)
