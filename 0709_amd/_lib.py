@@ -273,12 +273,15 @@ def require_device(*tensors: torch.Tensor | None, what: str) -> torch.device:
 
 
 _SAME_DEVICE = contextlib.nullcontext()
+# the device's index without the checks of torch.cuda.current_device() (a tensor on
+# a device means that all is set up)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(device: torch.device):
     """A context in which launches go to ``device`` (no cost where it is the
     current one already)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _CURRENT_DEVICE():
         return _SAME_DEVICE
     return torch.cuda.device(device)
 

@@ -325,10 +325,12 @@ struct Pages {
   }
 };
 
-// Joins the splits of a row block: one wave per row, its lanes over the dims.
+// Joins the splits of a row block: 16 lanes per row, each over D / 16 dims, four rows a
+// wave (one row a wave took three times as long over many rows: the chain from the
+// metadata to the partial states is walked once per wave, and it is what bounds this).
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a, int block_rows) {
-  constexpr int PL = D / 64;
+  constexpr int DL = D / 16;
   const atlas_paged_attn_t& p = a.p;
   const int item = blockIdx.x;
   const int rb = item % p.row_blocks;
@@ -337,40 +339,44 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a, 
   const Request r = read_request(p, b);
   const int row_start = rb * block_rows;
   const int rows = min(block_rows, r.q_len * a.group - row_start);
-  const int lr = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (lr >= rows) return;
-  const int lane = threadIdx.x & 63;
+  const int lr = blockIdx.y * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
+  if (lr >= rows) return;  // (whole rows: a row's lanes stay together)
   const Block k = plan_block(a, r, b, row_start, rows);
   if (k.splits <= 1) return;
   const float* ws = static_cast<const float*>(p.workspace);
   const int64_t nrows = int64_t(p.batch) * p.num_kv_heads * p.row_blocks * p.num_splits * block_rows;
   const int64_t row0 = int64_t(item) * p.num_splits * block_rows + lr;
   const float* lse_of = ws + nrows * D + row0;
+  const float* o_of = ws + row0 * D + lane * DL;
   float m = -INFINITY;
-  for (int s = lane; s < k.splits; s += 64) m = fmaxf(m, lse_of[int64_t(s) * block_rows]);
+  for (int s = lane; s < k.splits; s += 16) m = fmaxf(m, lse_of[int64_t(s) * block_rows]);
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  float sum = 0.f, acc[PL];
+  for (int x = 8; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+  float sum = 0.f;
+  f32x4 acc[DL / 4];
 #pragma unroll
-  for (int t = 0; t < PL; ++t) acc[t] = 0.f;
+  for (int t = 0; t < DL / 4; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < k.splits; ++s) {
     const float lse2 = lse_of[int64_t(s) * block_rows];
     const float f = lse2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(lse2 - m);
     sum += f;
 #pragma unroll
-    for (int t = 0; t < PL; ++t) acc[t] += f * ws[(row0 + int64_t(s) * block_rows) * D + lane * PL + t];
+    for (int t = 0; t < DL / 4; ++t)
+      acc[t] += f * *reinterpret_cast<const f32x4*>(o_of + int64_t(s) * block_rows * D + 4 * t);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int prow = row_start + lr, node = prow / a.group;
   const int head = h * a.group + (prow - node * a.group);
   uint16_t* out = static_cast<uint16_t*>(p.out) + int64_t(r.q0 + node) * p.out_stride_token +
-                  int64_t(head) * p.out_stride_head + lane * PL;
+                  int64_t(head) * p.out_stride_head + lane * DL;
   const bool bf16 = p.dtype == ATLAS_DTYPE_BF16;
-  if constexpr (PL == 2)
-    *reinterpret_cast<uint32_t*>(out) = bf16 ? pack_bf16(acc[0] * inv, acc[1] * inv) : pack_f16(acc[0] * inv, acc[1] * inv);
-  else
-    *out = uint16_t(bf16 ? pack_bf16(acc[0] * inv, 0.f) : pack_f16(acc[0] * inv, 0.f));
+#pragma unroll
+  for (int t = 0; t < DL / 4; ++t) {
+    const f32x4 x = acc[t] * inv;
+    *reinterpret_cast<w2*>(out + 4 * t) =
+        bf16 ? w2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])} : w2{pack_f16(x[0], x[1]), pack_f16(x[2], x[3])};
+  }
   if (p.lse != nullptr && lane == 0)
     p.lse[int64_t(r.q0 + node) * p.num_qo_heads + head] = sum == 0.f ? -INFINITY : (m + __builtin_log2f(sum)) * kPaLn2;
 }

@@ -102,14 +102,14 @@ def workspace_bytes(batch: int, kv_heads: int, head_dim: int, shape: tuple[bool,
     return 0 if splits == 1 else batch * kv_heads * blocks * splits * block_rows * (4 * head_dim + 4)
 
 
-def _i32(t: torch.Tensor, name: str, count: int, device: torch.device) -> torch.Tensor:
+def _i32(t: torch.Tensor, name: str, count: int, where: int) -> None:
+    """``t`` must hold ``count`` contiguous int32 on device ``where`` (``get_device()``)."""
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous int32 tensor")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    if t.get_device() != where:
+        raise ValueError(f"{name} is on {t.device}, not on the cache's device")
     if t.numel() != count:
         raise ValueError(f"{name} has {t.numel()} entries, expected {count}")
-    return t
 
 
 def cache_geometry(paged_kv_cache, kv_layout: str):
@@ -188,6 +188,7 @@ def paged_attention(
     base, v_offset, (page_stride, token_stride, head_stride), (pages, page_size, hkv, d) = cache_geometry(
         paged_kv_cache, kv_layout)
     device = _lib.require_device(q, base, what="paged attention")
+    where = q.get_device()
     if q.ndim != 3 or q.stride(-1) != 1:
         raise ValueError("q must be [nnz, Hq, D] with contiguous rows")
     nnz, hq, qd = q.shape
@@ -201,7 +202,7 @@ def paged_attention(
         s = kv_block_scales
         if s is None:
             raise ValueError("an 8-bit cache needs kv_block_scales")
-        if s.dtype != torch.float32 or tuple(s.shape) != (pages, 2, hkv) or s.device != device:
+        if s.dtype != torch.float32 or s.shape != (pages, 2, hkv) or s.get_device() != where:
             raise ValueError(f"kv_block_scales must be float32 [{pages}, 2, {hkv}] on {device}")
         ss = s.stride()
     elif base.dtype == q.dtype:
@@ -213,10 +214,10 @@ def paged_attention(
     batch = kv_last_page_len.numel()
     if batch == 0:
         raise ValueError("the batch must hold at least one request")
-    _i32(qo_indptr, "qo_indptr", batch + 1, device)
-    _i32(kv_indptr, "kv_indptr", batch + 1, device)
-    _i32(kv_last_page_len, "kv_last_page_len", batch, device)
-    _i32(kv_indices, "kv_indices", kv_indices.numel(), device)
+    _i32(qo_indptr, "qo_indptr", batch + 1, where)
+    _i32(kv_indptr, "kv_indptr", batch + 1, where)
+    _i32(kv_last_page_len, "kv_last_page_len", batch, where)
+    _i32(kv_indices, "kv_indices", kv_indices.numel(), where)
     mode, words = _lib.MASK_NONE, 1
     if tree_mask is not None:
         if causal or alibi_slopes is not None:
@@ -228,7 +229,7 @@ def paged_attention(
         if tree_mask.dtype != torch.int64 or not tree_mask.is_contiguous() or tree_mask.ndim > 2 or \
                 tree_mask.shape[0] < nnz or words < 1 or tree_mask.device != device:
             raise ValueError(f"tree_mask must be contiguous int64 [{nnz}] or [{nnz}, words] on {device}")
-        _i32(mask_col_start, "mask_col_start", batch, device)
+        _i32(mask_col_start, "mask_col_start", batch, where)
     elif causal:
         mode = _lib.MASK_CAUSAL
     if mode != _lib.MASK_CAUSAL and (window_left != -1 or prefix_lens is not None):
@@ -237,7 +238,7 @@ def paged_attention(
         raise ValueError("window_left must be -1 (none) or not negative")
     window_left = min(int(window_left), 1 << 30)
     if prefix_lens is not None:
-        _i32(prefix_lens, "prefix_lens", batch, device)
+        _i32(prefix_lens, "prefix_lens", batch, where)
     if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != hq
                                      or not alibi_slopes.is_contiguous() or alibi_slopes.device != device):
         raise ValueError(f"alibi_slopes must be contiguous float32 [{hq}] on {device}")

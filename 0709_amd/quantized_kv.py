@@ -109,6 +109,7 @@ def append_quantized(
     Rows are rounded to nearest, ties to even.  Infinities become the largest
     code and do not count for a scale; NaN stays NaN in e4m3 and becomes 0 in int8."""
     device, hkv, d, pages, page_size, args = _check_layers(layers, scales, kv_layout, "append_quantized")
+    where = layers[0].get_device()
     if len(k_src) != len(layers) or len(v_src) != len(layers):
         raise ValueError("one K and one V source per layer are required")
     first = k_src[0]
@@ -122,10 +123,10 @@ def append_quantized(
     batch = kv_last_page_len.numel()
     if batch == 0:
         raise ValueError("the batch must hold at least one request")
-    _i32(append_indptr, "append_indptr", batch + 1, device)
-    _i32(kv_indptr, "kv_indptr", batch + 1, device)
-    _i32(kv_last_page_len, "kv_last_page_len", batch, device)
-    _i32(kv_indices, "kv_indices", kv_indices.numel(), device)
+    _i32(append_indptr, "append_indptr", batch + 1, where)
+    _i32(kv_indptr, "kv_indptr", batch + 1, where)
+    _i32(kv_last_page_len, "kv_last_page_len", batch, where)
+    _i32(kv_indices, "kv_indices", kv_indices.numel(), where)
     if nnz == 0:
         return
     if max_append is None:
@@ -165,8 +166,9 @@ def commit_quantized(
     back when left out), rows past it stay where they are.  Requests must not
     share the pages they write to."""
     device, hkv, d, pages, page_size, args = _check_layers(layers, scales, kv_layout, "commit_quantized")
+    where = layers[0].get_device()
     for t, name in ((src_pos, "src_pos"), (dst_pos, "dst_pos")):
-        if t.dtype != torch.int64 or not t.is_contiguous() or t.device != device:
+        if t.dtype != torch.int64 or not t.is_contiguous() or t.get_device() != where:
             raise TypeError(f"{name} must be a contiguous int64 tensor on {device}")
     n = src_pos.numel()
     if dst_pos.numel() != n:
@@ -174,9 +176,9 @@ def commit_quantized(
     batch = item_indptr.numel() - 1
     if batch < 1:
         raise ValueError("the batch must hold at least one request")
-    _i32(item_indptr, "item_indptr", batch + 1, device)
-    _i32(kv_indptr, "kv_indptr", batch + 1, device)
-    _i32(kv_indices, "kv_indices", kv_indices.numel(), device)
+    _i32(item_indptr, "item_indptr", batch + 1, where)
+    _i32(kv_indptr, "kv_indptr", batch + 1, where)
+    _i32(kv_indices, "kv_indices", kv_indices.numel(), where)
     if n == 0:
         return
     if max_items is None:
