@@ -31,6 +31,7 @@ CACHE_16BIT = 0
 CACHE_E4M3 = 1
 CACHE_INT8 = 2
 QUANT_COMMIT_MAX_ITEMS = 64
+PAGED_ATTN_MAX_SOFT_CAP = 1024
 
 MASK_NONE = 0
 MASK_TREE = 1

@@ -43,7 +43,9 @@ extern "C" int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream) {
   ATLAS_REQUIRE(!p.single_token || p.mask_mode != 1, "single_token does not go with a tree mask");
   ATLAS_REQUIRE(p.row_blocks > 0 && p.num_splits > 0 && p.split_keys > 0 && p.split_keys % 64 == 0,
                 "row_blocks, num_splits and split_keys (a multiple of 64) must be positive");
-  ATLAS_REQUIRE(p.soft_cap >= 0.f, "soft_cap must not be negative");
+  ATLAS_REQUIRE(p.soft_cap == 0.f || (p.soft_cap >= 1e-37f && p.soft_cap <= ATLAS_PAGED_ATTN_MAX_SOFT_CAP),
+                "soft_cap must be 0 (none) or lie in [1e-37, %d]", ATLAS_PAGED_ATTN_MAX_SOFT_CAP);
+  ATLAS_REQUIRE(p.sm_scale >= -1e37f && p.sm_scale <= 1e37f, "sm_scale must lie in [-1e37, 1e37]");
   // rows and lanes load 16 bytes (V of an 8-bit cache or head_dim 64: less)
   const int es = p.cache == ATLAS_CACHE_16BIT ? 2 : 1;
   ATLAS_REQUIRE((reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && p.q_stride_token % 8 == 0 && p.q_stride_head % 8 == 0,
@@ -55,9 +57,10 @@ extern "C" int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream) {
                     p.token_stride % 16 == 0 && p.head_stride % 16 == 0,
                 "the cache must be 16-byte aligned with strides of 16 bytes");
   ATLAS_REQUIRE(p.token_stride >= p.head_dim * es, "token_stride does not cover a head's row");
-  if (p.num_indices * p.page_size >= (int64_t(1) << 31) || p.nnz >= (int64_t(1) << 31) / p.num_qo_heads ||
+  // (a tile past the last key still has positions below 2^31)
+  if (p.num_indices >= (int64_t(1) << 31) || p.num_indices * p.page_size >= (int64_t(1) << 31) - 4096 || p.nnz >= (int64_t(1) << 31) / p.num_qo_heads ||
       p.token_stride * p.page_size >= (int64_t(1) << 31)) {
-    set_error("page tables of 2^31 tokens or more, and pages of 2^31 bytes or more, are not supported");
+    set_error("page tables of 2^31 - 4096 tokens or more, and pages of 2^31 bytes or more, are not supported");
     return ATLAS_EUNSUPPORTED;
   }
   const int64_t blocks = int64_t(p.batch) * p.num_kv_heads * p.row_blocks;

@@ -77,6 +77,12 @@ __device__ __forceinline__ Request read_request(const atlas_paged_attn_t& p, int
   return r;
 }
 
+// Rows of a block that starts at packed row row_start (none: not positive).
+__device__ __forceinline__ int block_of(const PagedAttnArgs& a, const Request& r, int row_start) {
+  const int tokens = a.p.single_token ? min(r.q_len, 1) : r.q_len;
+  return min(a.p.block_rows, tokens * a.group - row_start);
+}
+
 // What a row block has to stream: the key chunks that some row of it may see, as
 // chunks of 64 keys 0 .. ca - 1 (the visible prefix) and cb .. ce - 1, and its splits.
 constexpr int kChunk = 64;
@@ -329,7 +335,7 @@ struct Pages {
 // wave (one row a wave took three times as long over many rows: the chain from the
 // metadata to the partial states is walked once per wave, and it is what bounds this).
 template <int D>
-__global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a, int block_rows) {
+__global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a) {
   constexpr int DL = D / 16;
   const atlas_paged_attn_t& p = a.p;
   const int item = blockIdx.x;
@@ -337,8 +343,8 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a, 
   const int h = item / p.row_blocks % p.num_kv_heads;
   const int b = item / p.row_blocks / p.num_kv_heads;
   const Request r = read_request(p, b);
-  const int row_start = rb * block_rows;
-  const int rows = min(block_rows, r.q_len * a.group - row_start);
+  const int block_rows = p.block_rows, row_start = rb * block_rows;
+  const int rows = block_of(a, r, row_start);
   const int lr = blockIdx.y * 16 + (threadIdx.x >> 4), lane = threadIdx.x & 15;
   if (lr >= rows) return;  // (whole rows: a row's lanes stay together)
   const Block k = plan_block(a, r, b, row_start, rows);

@@ -49,7 +49,7 @@ int launch_paged_attn(const PagedAttnArgs& a, hipStream_t stream) {
   int rc = launch_status("paged attention kernel");
   if (rc || p.num_splits == 1) return rc;
   const dim3 mgrid(static_cast<unsigned>(p.batch * p.num_kv_heads * p.row_blocks), p.block_rows / 16);
-  hipLaunchKernelGGL((paged_attn_merge_kernel<D>), mgrid, dim3(256), 0, stream, a, p.block_rows);
+  hipLaunchKernelGGL((paged_attn_merge_kernel<D>), mgrid, dim3(256), 0, stream, a);
   return launch_status("paged_attn_merge_kernel");
 }
 

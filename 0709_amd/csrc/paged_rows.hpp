@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   if (b >= p.batch) return;
   const Request r = read_request(p, b);
   const int row_start = rb * p.block_rows;
-  const int rows = min(p.block_rows, r.q_len * a.group - row_start);
+  const int rows = block_of(a, r, row_start);
   if (rows <= 0) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const Block k = plan_block(a, r, b, row_start, rows);

@@ -78,10 +78,9 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_stream_kernel(PagedAttnAr
   const int split = unit % p.num_splits;
   const int b = unit / p.num_splits;
   if (b >= p.batch) return;
-  Request r = read_request(p, b);
-  if (!MULTI) r.q_len = min(r.q_len, 1);
+  const Request r = read_request(p, b);
   const int row_start = rb * p.block_rows;
-  const int rows = min(p.block_rows, r.q_len * a.group - row_start);
+  const int rows = block_of(a, r, row_start);
   if (rows <= 0) return;
   const Block k = plan_block(a, r, b, row_start, rows);
   if (split >= k.splits) return;

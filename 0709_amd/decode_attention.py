@@ -354,8 +354,6 @@ class BatchDecodeWithPagedKVCacheWrapper:
         if logits_soft_cap is not None and float(logits_soft_cap) != (plan.soft_cap if scored else 0.0):
             if not scored:
                 raise NotImplementedError("plan with a logits_soft_cap, or with another option of scored attention")
-            if not 0.0 <= float(logits_soft_cap) < math.inf:
-                raise ValueError("logits_soft_cap must be finite and not negative")
             changes["soft_cap"] = float(logits_soft_cap)
         if sm_scale is not None:
             changes["sm_scale"] = float(sm_scale)

@@ -53,6 +53,11 @@ WHOLE_BYTES = 256 << 10
 # Many rows: the workgroups that run at once.
 BLOCK_WORKGROUPS = 512
 MAX_SPLITS = 256
+MAX_WORKGROUPS = 16384  # (splits of requests of a large batch, whose states take memory)
+
+# A capped score is cap * (1 - 2 / (1 + e^(2 s / cap))) in 32 bits, off by up to cap * 2^-21
+# however small the score: 2^-11 here, as much as a weight's rounding to fp16.
+MAX_SOFT_CAP = _lib.PAGED_ATTN_MAX_SOFT_CAP
 
 CACHE_CODES = {torch.float8_e4m3fn: _lib.CACHE_E4M3, torch.int8: _lib.CACHE_INT8}
 
@@ -91,7 +96,7 @@ def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_l
     else:
         keys = max(MIN_SPLIT_KEYS, -(-longest // max(1, CUS // items)))
         keys = min(keys, MAX_DECODE_SPLIT if single else MAX_STREAM_SPLIT)
-    keys = max(keys, -(-longest // MAX_SPLITS))
+    keys = max(keys, -(-longest // max(1, min(MAX_SPLITS, MAX_WORKGROUPS // items))))
     keys = -(-keys // 64) * 64
     return single, block_rows, blocks, -(-longest // keys), keys
 
@@ -170,9 +175,9 @@ def paged_attention(
     8-bit codes (float8_e4m3fn, int8) with ``kv_block_scales`` [pages, 2, Hkv]
     in float32.  The four metadata arrays are int32 device tensors.
 
-    ``max_q_len`` and ``max_kv_len`` size the launch: a request with more queries
-    than ``max_q_len`` gets its first rows only, one with more keys than
-    ``max_kv_len`` is right but slower.  Left out, they are read back from the
+    ``max_q_len`` and ``max_kv_len`` size the launch: of a request with more queries
+    than ``max_q_len`` only the first are sure to be computed, one with more keys
+    than ``max_kv_len`` is right but slower.  Left out, they are read back from the
     metadata, which waits for the device (and cannot be captured).
 
     Masks: none; ``causal`` with an optional ``window_left`` (keys more than that
@@ -244,8 +249,8 @@ def paged_attention(
         raise ValueError(f"alibi_slopes must be contiguous float32 [{hq}] on {device}")
     cap = 0.0 if logits_soft_cap is None else float(logits_soft_cap)
     scale = 1.0 / math.sqrt(d) if sm_scale is None else float(sm_scale)
-    if not (0.0 <= cap < math.inf and -math.inf < scale < math.inf):
-        raise ValueError("logits_soft_cap must be finite and not negative, sm_scale finite")
+    if not (cap == 0.0 or 1e-37 <= cap <= MAX_SOFT_CAP) or not abs(scale) <= 1e37:
+        raise ValueError(f"logits_soft_cap must be 0 (none) or lie in [1e-37, {MAX_SOFT_CAP}], sm_scale in [-1e37, 1e37]")
     if out is None:
         out = torch.empty((nnz, hq, d), dtype=q.dtype, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1 or out.device != device:
@@ -268,8 +273,8 @@ def paged_attention(
         raise ValueError("max_q_len and max_kv_len must not be negative")
     if max_q_len == 0:
         return (out, lse) if return_lse else out
-    max_q_len = min(int(max_q_len), nnz)
-    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, int(max_kv_len), tree=mode == _lib.MASK_TREE,
+    max_q_len, max_kv_len = min(int(max_q_len), nnz), min(int(max_kv_len), kv_indices.numel() * page_size)
+    shape = launch_shape(batch, hkv, hq // hkv, max_q_len, max_kv_len, tree=mode == _lib.MASK_TREE,
                          window_left=window_left, row_bytes=d * base.element_size(), quantized=s is not None, page_size=page_size)
     need = workspace_bytes(batch, hkv, d, shape)
     if need:

@@ -390,8 +390,9 @@ class BatchPrefillWithPagedKVCacheWrapper:
         window_left, cap = int(window_left), float(logits_soft_cap or 0.0)
         alibi = pos_encoding_mode == "ALIBI"
         masked = custom_mask is not None or packed_custom_mask is not None
-        if window_left < -1 or not 0.0 <= cap < math.inf:
-            raise ValueError("window_left must be -1 (none) or not negative, logits_soft_cap finite and not negative")
+        if window_left < -1 or not (cap == 0.0 or 1e-37 <= cap <= _lib.PAGED_ATTN_MAX_SOFT_CAP):
+            raise ValueError("window_left must be -1 (none) or not negative, logits_soft_cap 0 (none) or in "
+                             f"[1e-37, {_lib.PAGED_ATTN_MAX_SOFT_CAP}]")
         if window_left >= 0 and not causal:
             raise NotImplementedError("sliding windows need causal=True")
         if alibi and masked:

@@ -712,6 +712,9 @@ int atlas_candidate_select(const int64_t* parent_route_ids, const int64_t* stage
 #define ATLAS_CACHE_E4M3 1
 #define ATLAS_CACHE_INT8 2
 
+/* Largest soft cap: a capped score is off by up to cap * 2^-21. */
+#define ATLAS_PAGED_ATTN_MAX_SOFT_CAP 1024
+
 /* Arguments of atlas_paged_attn.  Pointers are device memory. */
 typedef struct {
   const void* q; /* [nnz, Hq, D], rows contiguous */
@@ -740,13 +743,13 @@ typedef struct {
   int32_t mask_mode; /* 0 none, 1 tree, 2 causal */
   int32_t mask_words;
   int32_t window_left; /* causal: keys below position - window_left are hidden; -1 none */
-  int32_t single_token; /* 1: no request has more than one query token (later ones are not written) */
+  int32_t single_token; /* 1: only the first query token of a request is computed (later ones are not written) */
   int32_t block_rows; /* packed rows (query token * group + head of the group) of a workgroup: a multiple of 16 up to 128, 16 with single_token */
   int32_t row_blocks; /* workgroups along a request's packed rows */
   int32_t num_splits; /* most key splits of a row block */
   int32_t split_keys; /* least keys of a split, a multiple of 64 */
   float sm_scale;
-  float soft_cap; /* 0: none; else scores become cap * tanh(score / cap) */
+  float soft_cap; /* 0: none; else in [1e-37, ATLAS_PAGED_ATTN_MAX_SOFT_CAP], and scores become cap * tanh(score / cap) */
 } atlas_paged_attn_t;
 
 /* Attention over a paged cache from device-side metadata alone (no plan):

@@ -30,8 +30,9 @@ def scored_attention(q, cache, qo_indptr, kv_indptr, kv_indices, kv_lens, *, pag
     The bounds: a weight rounded to 16 bits is off by weight_eps of itself, so the
     output by weight_eps * sum p |v|; a weight that falls below fp16's range by 2^-24 of the
     largest V; a score summed in fp32 over D products by (D + 8) 2^-24 of the sum of
-    their magnitudes (doubled for the exponent's own error), which changes every
-    weight by as much; the result is rounded once to q's type."""
+    their magnitudes (doubled for the exponent's own error), a cap c computed as
+    c - 2 c / (1 + e) by c 2^-21 (e is off by 2^-22 of itself, which moves the quotient by c / 2 of
+    that, and the reciprocal by 2^-23 of up to 2 c), which changes every weight by as much; the result is rounded once to q's type."""
     hq, d = q.shape[1], q.shape[2]
     sm = d ** -0.5 if sm_scale is None else sm_scale
     outs, lses, tols, ltols = [], [], [], []
@@ -71,7 +72,7 @@ def scored_attention(q, cache, qo_indptr, kv_indptr, kv_indices, kv_lens, *, pag
                 seen = vis[i].nonzero()[:, 0]
                 o[h, i] = p[h, i, seen] @ v[seen, h]
                 a[h, i] = p[h, i, seen] @ v[seen, h].abs()
-        ds = 2 * (d + 8) * 2.0 ** -24 * (mag.amax(-1) if n_keys else torch.zeros((hq, n))) + 2.0 ** -20
+        ds = 2 * (d + 8) * 2.0 ** -24 * (mag.amax(-1) if n_keys else torch.zeros((hq, n))) + 2.0 ** -20 + soft_cap * 2.0 ** -21
         vmax = v[torch.isfinite(v)].abs().max() if n_keys else 0.0
         outs.append(o.transpose(0, 1))
         lses.append(lse.transpose(0, 1))

@@ -364,3 +364,53 @@ def test_nan_scores_reach_their_rows(dev):
         out, lse = call(dev, s)
         assert torch.isnan(out[0, 4:]).all() and torch.isnan(lse[0, 4:]).all()
         assert torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1]).all() and torch.isfinite(lse[1]).all()
+
+
+@pytest.mark.parametrize("cache", ["same", torch.int8], ids=str)
+@pytest.mark.parametrize("opts", [dict(causal=True), dict(causal=True, window_left=20), dict()])
+def test_more_tokens_than_stated(dev, cache, opts):
+    """max_q_len=1 over requests of several tokens: the first token of each is right
+    (at its own position), the others stay as they were."""
+    s = build(171, [3, 1, 2], [700, 1300, 5], cache=cache)
+    out, lse = torch.full(s["q"].shape, 7.0, dtype=torch.bfloat16, device=dev), torch.full((6, 8), 7.0, device=dev)
+    call(dev, s, max_q_len=1, out=out, lse=lse, **opts)
+    want, wl, tol, ltol = scored_attention(s["q"], s["cache"], s["qo"], s["kvp"], s["table"], s["kv_lens"], page_size=16,
+                                           kv_layout="NHD", scales=s["scales"], weight_eps=weight_eps(s), **opts)
+    first = [0, 3, 4]
+    assert ((out.cpu().double() - want).abs() <= tol)[first].all()
+    assert ((lse.cpu().double() - wl).abs() <= ltol)[first].all()
+    for row in (1, 2, 5):
+        assert bool((out[row] == 7).all()) and bool((lse[row] == 7).all())
+
+
+@pytest.mark.parametrize("cache", CACHES, ids=str)
+@pytest.mark.parametrize("hq,hkv", [(40, 2), (17, 1), (6, 2), (71, 1)])
+@pytest.mark.parametrize("n", [1, 2, 9])
+def test_group_sizes(dev, cache, hq, hkv, n):
+    """Groups of more query heads than a row tile, and odd ones."""
+    s = build(181, [n, 1], [300, 2000], hq=hq, hkv=hkv, cache=cache, ps=32)
+    check(s, call(dev, s, causal=True), causal=True)
+
+
+@pytest.mark.parametrize("cache", ["same", torch.float8_e4m3fn], ids=str)
+@pytest.mark.parametrize("prefix", [0, 5, 700])
+def test_windows_behind_long_prefixes(dev, cache, prefix):
+    """The splits are sized for the window; a prefix that is longer is still whole."""
+    s = build(191, [1, 1, 4], [900, 3000, 1500], cache=cache)
+    pre = torch.tensor([prefix] * 3, dtype=torch.int32)
+    check(s, call(dev, s, causal=True, window_left=40, prefix_lens=pre.to(dev)), causal=True, window_left=40, prefix_lens=pre)
+
+
+def test_extreme_caps(dev):
+    """The smallest and the largest cap that are taken."""
+    s = build(201, [1, 3], [300, 50])
+    for cap in (1e-37, 1e-3, 1024.0):
+        check(s, call(dev, s, causal=True, logits_soft_cap=cap), causal=True, soft_cap=cap)
+
+
+def test_large_batches_and_lengths_stated(dev):
+    """Many requests, and a max_kv_len far above any: few splits are left, and the rows are the same."""
+    s = build(211, [1] * 80, [17 * i % 400 for i in range(80)], hq=8, hkv=2, cache=torch.int8)
+    a, b = call(dev, s), call(dev, s, max_kv_len=1 << 40)
+    check(s, a)
+    check(s, b)

@@ -47,7 +47,8 @@ def attn_args(**changes):
     (dict(voff=8), EINVAL), (dict(token=264), EINVAL), (dict(token=128), EINVAL), (dict(head=8), EINVAL),
     (dict(indices=1 << 27), EUNSUPPORTED), (dict(nnz=1 << 30), EUNSUPPORTED), (dict(token=1 << 27), EUNSUPPORTED),
     (dict(splits=1 << 22), EUNSUPPORTED), (dict(splits=4), EINVAL), (dict(splits=4, ws=1 << 20, ws_bytes=100), EINVAL),
-    (dict(splits=4, ws=(1 << 20) + 4, ws_bytes=1 << 30), EINVAL), (dict(cap=math.nan), EINVAL),
+    (dict(splits=4, ws=(1 << 20) + 4, ws_bytes=1 << 30), EINVAL), (dict(cap=math.nan), EINVAL), (dict(cap=1e-40), EINVAL), (dict(cap=1025.0), EINVAL), (dict(sm=math.nan), EINVAL),
+    (dict(sm=-2e37), EINVAL), (dict(indices=(1 << 27) - 256), EUNSUPPORTED),
 ])
 def test_attention_entry_refuses(changes, code):
     lib, L = pkg("_lib").load(), pkg("_lib")
@@ -195,11 +196,12 @@ SCALES = torch.ones((5, 2, 2))
     (dict(causal=True, window_left=-2), ValueError), (dict(causal=True, prefix_lens=i32([1])), ValueError),
     (dict(alibi_slopes=torch.ones(3)), ValueError), (dict(alibi_slopes=torch.ones(4).double()), ValueError),
     (dict(logits_soft_cap=-1.0), ValueError), (dict(logits_soft_cap=math.inf), ValueError),
-    (dict(logits_soft_cap=math.nan), ValueError), (dict(sm_scale=math.inf), ValueError), (dict(sm_scale=math.nan), ValueError),
+    (dict(logits_soft_cap=math.nan), ValueError), (dict(logits_soft_cap=1e-50), ValueError),
+    (dict(logits_soft_cap=1025.0), ValueError), (dict(sm_scale=1e39), ValueError), (dict(sm_scale=math.inf), ValueError), (dict(sm_scale=math.nan), ValueError),
     (dict(out=torch.zeros((2, 4, 128))), ValueError), (dict(out=torch.zeros((1, 4, 128), dtype=BF16)), ValueError),
     (dict(lse=torch.zeros((2, 4), dtype=BF16)), ValueError), (dict(lse=torch.zeros((4, 2)).T), ValueError),
     (dict(max_q_len=-1), ValueError), (dict(max_kv_len=-1), ValueError),
-    (dict(max_kv_len=9000, workspace=torch.zeros(10, dtype=torch.uint8)), ValueError),
+    (dict(max_kv_len=9000, kv_indices=i32([0] * 600), workspace=torch.zeros(10, dtype=torch.uint8)), ValueError),
 ])
 def test_attention_refuses(lib, changes, error):
     with pytest.raises(error):
@@ -216,6 +218,8 @@ def test_attention_calls(lib):
     assert len(lib.calls) == 1
     attn_call(paged_kv_cache=CODES, kv_block_scales=SCALES, causal=True, window_left=1 << 40)
     assert len(lib.calls) == 2
+    attn_call(max_q_len=1 << 40, max_kv_len=1 << 40)  # (no more than the tokens and the table hold)
+    assert len(lib.calls) == 3
 
 
 def append_call(**changes):
@@ -303,7 +307,7 @@ def test_launch_shapes_are_accepted(batch, hkv, group, tree, quantized, page):
             assert per % 64 == 0 and 1 <= splits <= pa.MAX_SPLITS and splits * per >= keys
             if not single and block > 16 and page % 16:
                 assert rows * group > pa.MAX_STREAM_ROWS
-            assert batch * hkv * blocks * splits < 1 << 23
+            assert splits == 1 or batch * hkv * blocks * splits <= pa.MAX_WORKGROUPS
 
 
 def test_window_sizes_the_splits():
