@@ -38,8 +38,8 @@ extern "C" int atlas_paged_attn(const atlas_paged_attn_t* args, void* stream) {
   ATLAS_REQUIRE(p.mask_mode == 2 || (p.window_left < 0 && p.prefix_lens == nullptr),
                 "windows and prefixes go with the causal mask");
   ATLAS_REQUIRE(p.mask_mode != 1 || p.alibi_slopes == nullptr, "a distance bias does not go with a tree mask");
-  ATLAS_REQUIRE(p.block_rows > 0 && p.block_rows % 16 == 0 && p.block_rows <= (p.single_token ? 16 : 128),
-                "block_rows must be a multiple of 16, up to 128 (16 for single tokens), got %d", p.block_rows);
+  ATLAS_REQUIRE(p.block_rows > 0 && p.block_rows % 16 == 0 && p.block_rows <= (p.single_token ? 16 : 256),
+                "block_rows must be a multiple of 16, up to 256 (16 for single tokens), got %d", p.block_rows);
   ATLAS_REQUIRE(!p.single_token || p.mask_mode != 1, "single_token does not go with a tree mask");
   ATLAS_REQUIRE(p.row_blocks > 0 && p.num_splits > 0 && p.split_keys > 0 && p.split_keys % 64 == 0,
                 "row_blocks, num_splits and split_keys (a multiple of 64) must be positive");

@@ -35,7 +35,7 @@ void launch_paged_kernel(const PagedAttnArgs& a, hipStream_t stream) {
       }
     }
   }
-  hipLaunchKernelGGL((paged_rows_kernel<KIND, D, PAGE16, SCORED>), grid, block, 0, stream, a);
+  hipLaunchKernelGGL((paged_rows_kernel<KIND, D, PAGE16, SCORED>), grid, dim3(kRowThreads), 0, stream, a);
 }
 
 template <int KIND, int D>

@@ -1,12 +1,18 @@
 // Paged attention for many packed rows: prompts' chunks and wide draft trees.
 //
-// A workgroup of four waves takes up to 128 packed rows of one KV head and one split
-// of the request's keys.  Tiles of 32 keys (64 at head_dim 64) go from HBM through
-// registers into LDS as 16-bit rows (8-bit codes are converted on the way, once for all
-// rows): one tile is computed from one of two stages, the next is written to the
-// other, and two more are on their way.  Row tiles of 16 go round the waves; K's operand is a
-// 16-byte LDS read, V's two transposing reads.  A row's 16-byte granules are swapped
-// by the key so that neither the writes nor either kind of read meets in a bank.
+// A workgroup of eight waves takes up to 256 packed rows of one KV head and one split
+// of the request's keys.  Tiles of 64 keys go from HBM through registers into LDS as
+// 16-bit rows (8-bit codes are converted on the way, once for all rows): one tile is
+// computed from one of two stages, the next is written to the other, and one more (two
+// at head_dim 64) is on its way.  Row tiles of 16 go round the waves, two for each; K's
+// operand is a 16-byte LDS read, V's two transposing reads.  A row's 16-byte granules
+// are swapped by the key so that neither the writes nor either kind of read meets in a
+// bank.
+//
+// Bound by the vector instructions of the softmax (per score of a lane about ten, the
+// exponential counting for four) beside the matrix instructions, which two waves of a SIMD
+// overlap in part.  Four waves on 128 rows, two such workgroups to a CU, or tiles of 32 keys
+// took 3 to 10 % longer: each wave then has more of the staging to do, or meets more barriers.
 #pragma once
 
 #include "paged_attn.hpp"
@@ -28,6 +34,9 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+constexpr int kRowWaves = 8;
+constexpr int kRowThreads = 64 * kRowWaves;
+
 template <int N>
 using Stage = std::integral_constant<int, N>;
 
@@ -35,12 +44,12 @@ using Stage = std::integral_constant<int, N>;
 // wave-uniform; other page sizes look every key up.  SCORED: scores may be capped or
 // biased, or their factor negative.
 template <int KIND, int D, bool PAGE16, bool SCORED>
-__global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kRowThreads, 2) void paged_rows_kernel(PagedAttnArgs a) {
   typedef Cache<KIND> C;
   typedef typename C::frag frag;
   constexpr bool Q8 = C::kQuant;
   constexpr int RT = 2;                    // row tiles of a wave
-  constexpr int TK = D == 128 ? 32 : 64;  // keys of a tile
+  constexpr int TK = 64;                   // keys of a tile
   constexpr int SUB = kChunk / TK;         // tiles of a chunk
   constexpr int NT = TK / 16;              // its 16-key tiles
   constexpr int KS = D / 32;               // steps of the score product
@@ -48,8 +57,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   constexpr int RB = D * 2;                // bytes of an LDS row
   constexpr int GR = RB / 16;              // its granules
   constexpr int HALF = TK * RB;            // K's or V's half of a stage
-  constexpr int GG = D * C::kBytes / 16;   // 16-byte pieces of a row in the cache
-  constexpr int NL = TK * GG / kPaThreads; // pieces a thread carries, of K and of V
+  constexpr int PB = 8 * C::kBytes;        // bytes of eight values in the cache, a granule in LDS
   constexpr int KSW = GR - 1;              // granule swaps: K by key, V by key pairs
   constexpr int VSW = GR / 2 - 1;
   const atlas_paged_attn_t& p = a.p;
@@ -99,7 +107,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   int node_of[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int row = (wave + 4 * rt) * 16 + r16;
+    const int row = (wave + kRowWaves * rt) * 16 + r16;
     const bool ok = row < rows;
     const int prow = row_start + (ok ? row : 0);
     node_of[rt] = prow / a.group;
@@ -167,15 +175,18 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       win_vs = sc[p.scale_stride_kv];
     }
   };
-  // Piece j of a thread: row (j * 256 + tid) / GG of the tile, piece tid % GG of it.
-  const int piece = tid % GG, prow0 = tid / GG;
-  constexpr int RSTEP = kPaThreads / GG;  // rows between a thread's pieces
-  static_assert(RSTEP % 16 == 0, "a thread's pieces have the same place in their 16-key tiles");
-  const uint32_t piece_at = uint32_t((prow0 & 15) * ts + piece * 16);
-  constexpr int KTH = kPaThreads / TK;  // threads per key
-  constexpr int SETS = 2;               // tiles in flight in registers
+  // A thread carries eight values of NL K rows and of as many V rows of a tile: those of
+  // granule `gr` of rows `row`, `row` + RSTEP ..
+  constexpr int NL = TK * GR / kRowThreads, RSTEP = kRowThreads / GR;
+  static_assert(RSTEP % 16 == 0, "a thread's rows have the same place in their 16-key tiles");
+  typedef std::conditional_t<Q8, w2, w4> Piece;
+  const int gr = tid % GR, row = tid / GR;
+  const int kt_of = wave * (64 / GR) >> 4;  // (a wave's rows lie in one 16-key tile)
+  const uint32_t piece_at = uint32_t((row & 15) * ts + gr * PB);
+  constexpr int KTH = kRowThreads / TK;  // threads per key
+  constexpr int SETS = 2 / NL;           // tiles in flight in registers
   struct Raw {
-    w4 k[NL], v[NL];
+    Piece k[NL], v[NL];
     float ks, vs;  // scales of 16-key tile lane % NT; other page sizes: of key tid / KTH
   };
   // Keys outside [lo, hi) of the tile's part repeat its nearest key.
@@ -187,22 +198,19 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
       if constexpr (PAGE16) {
-        // (a wave's rows of one piece lie in one 16-key tile)
-        const int kt = (j * RSTEP + wave * (64 / GG)) >> 4;
+        const int kt = kt_of + j * RSTEP / 16;
         const int64_t row0 = Pages::tile_row(win_rows, (c - win0) * NT + kt);
         uint32_t off = piece_at;
-        if (!whole) {
-          const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
-          off = uint32_t((key - Pages::tile_key(kb, kt, lo, hi)) * ts + piece * 16);
-        }
-        x.k[j] = *reinterpret_cast<const w4*>(kbase + row0 + off);
-        x.v[j] = *reinterpret_cast<const w4*>(vbase + row0 + off);
+        if (!whole)
+          off = uint32_t((min(max(kb + row + j * RSTEP, lo), hi) - Pages::tile_key(kb, kt, lo, hi)) * ts + gr * PB);
+        x.k[j] = *reinterpret_cast<const Piece*>(kbase + row0 + off);
+        x.v[j] = *reinterpret_cast<const Piece*>(vbase + row0 + off);
       } else {
-        const int key = min(max(kb + j * RSTEP + prow0, lo), hi);
+        const int key = min(max(kb + row + j * RSTEP, lo), hi);
         const int slot = slot_of(a, key);
-        const int64_t at = pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts + piece * 16;
-        x.k[j] = *reinterpret_cast<const w4*>(kbase + at);
-        x.v[j] = *reinterpret_cast<const w4*>(vbase + at);
+        const int64_t at = pages.valid(pages.ids[slot]) * p.page_stride + int64_t(key - slot * page_size) * ts + gr * PB;
+        x.k[j] = *reinterpret_cast<const Piece*>(kbase + at);
+        x.v[j] = *reinterpret_cast<const Piece*>(vbase + at);
       }
     }
     if constexpr (Q8 && PAGE16) {
@@ -225,7 +233,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   // Infinities and NaN in V rows that a row does not see must not reach it (0 * inf):
   // in tiles with hidden keys they are stored as zeros and marked, and the rows
   // that see them get them from the marks.
-  auto take_out = [&](frag v, int st, int row, int gr, uint32_t& odd) __attribute__((always_inline)) {
+  auto take_out = [&](frag v, int st, int at, uint32_t& odd) __attribute__((always_inline)) {
     uint32_t up = 0, dn = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -235,50 +243,35 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
       dn |= ((d >> 15 & 1u) | (d >> 30 & 2u)) << (2 * w);
       odd |= u | d;
     }
-    up_lds[st][row * (D / 8) + gr] = uint8_t(up);
-    dn_lds[st][row * (D / 8) + gr] = uint8_t(dn);
+    up_lds[st][at * GR + gr] = uint8_t(up);
+    dn_lds[st][at * GR + gr] = uint8_t(dn);
     return v;
   };
+  const int k_to = row * RB + ((gr ^ (row & KSW)) << 4), v_to = row * RB + ((gr ^ ((row & VSW) << 1)) << 4);
   auto store = [&](const Raw& x, auto st_tag, int c) __attribute__((always_inline)) {
     constexpr int st = decltype(st_tag)::value;
-    char* kd = lds[st];
-    char* vd = lds[st] + HALF;
-    frag vv[Q8 ? 2 * NL : NL];
+    frag vv[NL];
 #pragma unroll
     for (int j = 0; j < NL; ++j) {
-      const int row = j * RSTEP + prow0;
-      if constexpr (!Q8) {
-        *reinterpret_cast<w4*>(kd + row * RB + ((piece ^ (row & KSW)) << 4)) = x.k[j];
-        vv[j] = x.v[j];
+      frag kk;
+      if constexpr (Q8) {
+        kk = C::keys8(x.k[j][0], x.k[j][1]);
+        vv[j] = C::keys8(x.v[j][0], x.v[j][1]);
       } else {
-        // (half of the pieces write their second granule first: eight lanes then write eight
-        // different residues of granules, which share no bank)
-        const bool swap = piece & (GG / 2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bool second = swap != (e == 1);
-          *reinterpret_cast<frag*>(kd + row * RB + (((2 * piece + second) ^ (row & KSW)) << 4)) =
-              C::keys8(second ? x.k[j][2] : x.k[j][0], second ? x.k[j][3] : x.k[j][1]);
-          vv[2 * j + e] = C::keys8(second ? x.v[j][2] : x.v[j][0], second ? x.v[j][3] : x.v[j][1]);
-        }
+        kk = x.k[j];
+        vv[j] = x.v[j];
       }
+      *reinterpret_cast<frag*>(lds[st] + k_to + j * RSTEP * RB) = kk;
     }
-    auto granule = [&](int j) __attribute__((always_inline)) {
-      return Q8 ? 2 * piece + int(bool(piece & (GG / 2)) != bool(j & 1)) : piece;
-    };
     if (KIND != kCacheInt8 && masked_tile(key_of(c))) {
       // (the marks of a tile are whole: every thread writes its part, whether it has some or not)
       uint32_t odd = 0;
 #pragma unroll
-      for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j)
-        vv[j] = take_out(vv[j], st, (Q8 ? j >> 1 : j) * RSTEP + prow0, granule(j), odd);
+      for (int j = 0; j < NL; ++j) vv[j] = take_out(vv[j], st, row + j * RSTEP, odd);
       if (odd) strange_lds[st] = c + 1;
     }
 #pragma unroll
-    for (int j = 0; j < (Q8 ? 2 * NL : NL); ++j) {
-      const int row = (Q8 ? j >> 1 : j) * RSTEP + prow0, gr = granule(j);
-      *reinterpret_cast<frag*>(vd + row * RB + ((gr ^ ((row & VSW) << 1)) << 4)) = vv[j];
-    }
+    for (int j = 0; j < NL; ++j) *reinterpret_cast<frag*>(lds[st] + HALF + v_to + j * RSTEP * RB) = vv[j];
     if constexpr (Q8 && PAGE16) {
       if (tid < NT) {
         scale_lds[st][0][tid] = x.ks;
@@ -527,11 +520,11 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
     int c = c0;
     while (c < c1) {
       for (; c < c1 && masked_pair(c); c += 2) {
-        step(std::true_type{}, Stage<0>{}, x[1], c);
+        step(std::true_type{}, Stage<0>{}, x[SETS - 1], c);
         if (c + 1 < c1) step(std::true_type{}, Stage<1>{}, x[0], c + 1);
       }
       for (; c < c1 && !masked_pair(c); c += 2) {
-        step(std::false_type{}, Stage<0>{}, x[1], c);
+        step(std::false_type{}, Stage<0>{}, x[SETS - 1], c);
         if (c + 1 < c1) step(std::false_type{}, Stage<1>{}, x[0], c + 1);
       }
     }
@@ -541,7 +534,7 @@ __global__ __launch_bounds__(kPaThreads, 2) void paged_rows_kernel(PagedAttnArgs
   const int64_t item = (int64_t(b) * p.num_kv_heads + h) * p.row_blocks + rb;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int lr = (wave + 4 * rt) * 16 + r16;
+    const int lr = (wave + kRowWaves * rt) * 16 + r16;
     const float sum = groups_sum(l_run[rt]);
     if (lr >= rows) continue;
     const float inv = (sum == 0.f ? 0.f : 1.f / sum) * (Q8 ? vref : 1.f);

@@ -39,8 +39,14 @@ DECODE_ROWS = 16
 STREAM_ROWS_8BIT = 48
 STREAM_ROWS_16BIT = 32
 STREAM_ROWS_PAGES = 16
-WIDE_ROWS = 128
-# Requests of more packed rows than this take the kernel of many rows.
+WIDE_ROWS = 256
+# Requests whose rows make several such blocks stream their keys once for each; the kernel
+# of many rows reads them once and takes longer to start.  It is taken when the blocks
+# would stream more keys than this in all (16 bits, one request of 1000 keys and 96 rows: 13.6 us
+# against 19.8; 8 of 4096 keys: 87 against 51), 8-bit caches up to MAX_STREAM_ROWS never
+# (8 x 4096 keys, 192 rows: 60 us against 66; 240 rows: 79 against 71).
+STREAM_KEYS_16BIT = 1 << 17
+STREAM_KEYS_8BIT = 1 << 19
 MAX_STREAM_ROWS = 192
 # Single tokens and few rows: splits as long as one per CU makes them, between these
 # (short splits even out requests of different lengths); a request of a single token whose
@@ -51,7 +57,7 @@ MAX_DECODE_SPLIT = 1536
 MAX_STREAM_SPLIT = 4096
 WHOLE_BYTES = 256 << 10
 # Many rows: the workgroups that run at once.
-BLOCK_WORKGROUPS = 512
+BLOCK_WORKGROUPS = 256
 MAX_SPLITS = 256
 MAX_WORKGROUPS = 16384  # (splits of requests of a large batch, whose states take memory)
 
@@ -81,10 +87,12 @@ def launch_shape(batch: int, kv_heads: int, group: int, max_q_len: int, max_kv_l
     rows = max(1, max_q_len * group)
     if single:
         most_rows = DECODE_ROWS
-    elif rows <= MAX_STREAM_ROWS:
-        most_rows = STREAM_ROWS_PAGES if page_size % 16 else (STREAM_ROWS_8BIT if quantized else STREAM_ROWS_16BIT)
     else:
-        most_rows = WIDE_ROWS
+        most_rows = STREAM_ROWS_PAGES if page_size % 16 else (STREAM_ROWS_8BIT if quantized else STREAM_ROWS_16BIT)
+        streamed = -(-rows // most_rows) * batch * kv_heads * max_kv_len
+        if rows > most_rows and streamed > (STREAM_KEYS_8BIT if quantized else STREAM_KEYS_16BIT) and not (
+                quantized and rows <= MAX_STREAM_ROWS and page_size % 16 == 0):
+            most_rows = WIDE_ROWS
     blocks = -(-rows // most_rows)
     block_rows = 16 * -(-rows // (16 * blocks))
     items = batch * kv_heads * blocks

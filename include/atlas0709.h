@@ -744,7 +744,7 @@ typedef struct {
   int32_t mask_words;
   int32_t window_left; /* causal: keys below position - window_left are hidden; -1 none */
   int32_t single_token; /* 1: only the first query token of a request is computed (later ones are not written) */
-  int32_t block_rows; /* packed rows (query token * group + head of the group) of a workgroup: a multiple of 16 up to 128, 16 with single_token */
+  int32_t block_rows; /* packed rows (query token * group + head of the group) of a workgroup: a multiple of 16 up to 256, 16 with single_token */
   int32_t row_blocks; /* workgroups along a request's packed rows */
   int32_t num_splits; /* most key splits of a row block */
   int32_t split_keys; /* least keys of a split, a multiple of 64 */

@@ -41,7 +41,7 @@ def attn_args(**changes):
     (dict(mode=3), EINVAL), (dict(mode=1, single=0), EINVAL), (dict(mode=1, tree=8, col=8), EINVAL),
     (dict(mode=1, tree=8, col=8, words=0, single=0), EINVAL), (dict(window=3), EINVAL), (dict(prefix=8), EINVAL),
     (dict(mode=1, tree=8, col=8, single=0, slopes=8), EINVAL), (dict(rows=8), EINVAL), (dict(rows=32), EINVAL),
-    (dict(rows=144, single=0), EINVAL), (dict(blocks=0), EINVAL), (dict(splits=0), EINVAL), (dict(keys=100), EINVAL),
+    (dict(rows=272, single=0), EINVAL), (dict(blocks=0), EINVAL), (dict(splits=0), EINVAL), (dict(keys=100), EINVAL),
     (dict(keys=0), EINVAL), (dict(cap=-1.0), EINVAL), (dict(q=(1 << 20) + 2), EINVAL), (dict(qst=4), EINVAL),
     (dict(out=(1 << 20) + 8), EINVAL), (dict(osh=4), EINVAL), (dict(kv=(1 << 20) + 8), EINVAL), (dict(page=8), EINVAL),
     (dict(voff=8), EINVAL), (dict(token=264), EINVAL), (dict(token=128), EINVAL), (dict(head=8), EINVAL),
@@ -303,10 +303,8 @@ def test_launch_shapes_are_accepted(batch, hkv, group, tree, quantized, page):
             single, block, blocks, splits, per = pa.launch_shape(batch, hkv, group, rows, keys, tree=tree,
                                                                  quantized=quantized, page_size=page)
             assert single == (rows <= 1 and not tree)
-            assert block % 16 == 0 and 16 <= block <= (16 if single else 128) and block * blocks >= rows * group
+            assert block % 16 == 0 and 16 <= block <= (16 if single else 256) and block * blocks >= rows * group
             assert per % 64 == 0 and 1 <= splits <= pa.MAX_SPLITS and splits * per >= keys
-            if not single and block > 16 and page % 16:
-                assert rows * group > pa.MAX_STREAM_ROWS
             assert splits == 1 or batch * hkv * blocks * splits <= pa.MAX_WORKGROUPS
 
 
