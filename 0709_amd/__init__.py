@@ -8,6 +8,9 @@ Drop-in modules (same names and call signatures as the reference package
   ``write_suffix_kv``, paged prefix conversion, the verify-attention plan;
 * ``tree_attention``         -- ``BatchPrefillWithPagedKVCacheWrapper`` (plan/run);
 * ``kv_ops``                 -- all-layer append, move (COW) and commit kernels;
+* ``paged_attention``        -- attention from device-side metadata: 16-bit and 8-bit
+  caches, caps, windows, distance bias, draft trees;
+* ``quantized_kv``           -- 8-bit caches: quantising append, route commit;
 * ``flashinfer_paged``       -- paged metadata, route-pool bridge, native pools;
 * ``target_runtime``         -- Target commit / capacity / scoring / selection.
 

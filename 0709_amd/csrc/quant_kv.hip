@@ -74,7 +74,9 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // threads: the rows are read once, into registers (kHeld vectors of 8 values a
 // thread; what a large page holds beyond that is read twice), their largest value
 // gives the scale, and the codes follow.  Bound by the bytes: 2 read and 1 written
-// per value.
+// per value (8 prompts of 2048 tokens into 16 layers: 143 us for 647 MB, 4.5 TB/s; reading the
+// rows a second time, for the codes, took 150).  A decode step's rows are one chain of
+// loads, about 5 us.
 template <int CACHE, bool BF16, int UNIT>
 __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(QuantTables qt, RowTables st, QuantGeom g,
                                                                              Appends a) {
@@ -202,7 +204,9 @@ __device__ __forceinline__ int64_t shuffle64(int64_t v, int lane) {
 // Lane i holds item i: its rows' offsets, its blocks' scales, whether it is the first
 // item of its destination block; what the others need of it goes through readlane and
 // shuffles.  A few hundred bytes per wave: bound by the chain of loads from the
-// positions to the rows, so every wave of a call should be in flight at once.
+// positions to the rows, so every wave of a call should be in flight at once: 4.4 us for one
+// request, 17 us for 32 requests and 32 layers (16384 waves).  With the rows and tables in LDS, one
+// wave a workgroup, those took 7.5 and 29 us.
 template <int CACHE, int D>
 __global__ __launch_bounds__(64 * kCommitWaves) void kv_commit_quantized_kernel(QuantTables qt, QuantGeom g, Commits c) {
   constexpr int kLanes = D / 16;        // lanes of 16 codes per row

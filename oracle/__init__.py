@@ -24,6 +24,10 @@ Pinning (what each function is checked against in ``tests/``):
                              SGLang's own allocator is absent: parity unpinned
                              against it (only against this restated policy).
 * ``scoring``             -- reference literals (test_target_kv_commit.py:76-367)
+* ``scored_attention``    -- closed form in 64 bits (no counterpart in the reference),
+                             with bounds on a 16-bit kernel's difference
+* ``quantized``           -- the 8-bit append and commit by their definitions, row by
+                             row in 64 bits (no counterpart in the reference)
 * ``frontier``            -- reference literals of the frontier selection tests
                              (test_paged_frontier_selection.py:79-130, :189-275),
                              the Python-object order by brute force (utils.py:27-43),
