@@ -13,6 +13,7 @@ namespace {
 typedef uint32_t w4 __attribute__((ext_vector_type(4)));
 typedef uint32_t w2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u2 __attribute__((ext_vector_type(2)));
 
 constexpr int kAppendThreads = 256;
 constexpr int kHeld = 8;  // vectors of a thread's rows in registers
@@ -60,6 +61,20 @@ __device__ __forceinline__ void to_floats(w4 v, float (&f)[8]) {
   }
 }
 
+// Largest magnitude so far, as bits, of the even and the odd values: those of finite
+// 16-bit values are in their order.  (In fp32 the compiler keeps the values for the codes
+// as well, and half as many waves fit.)
+template <bool BF16>
+__device__ __forceinline__ u2 largest(u2 most, w4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bad = ((v[i] & (BF16 ? 0x7f807f80u : 0x7c007c00u)) + (BF16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+    const uint32_t x = v[i] & 0x7fff7fffu & ~((bad << 1) - (bad >> 15));
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(u2, x));
+  }
+  return most;
+}
+
 // Four codes under a scale that is 1 / ratio times theirs.
 template <int CACHE>
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
@@ -74,8 +89,8 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // threads: the rows are read once, into registers (kHeld vectors of 8 values a
 // thread; what a large page holds beyond that is read twice), their largest value
 // gives the scale, and the codes follow.  Bound by the bytes: 2 read and 1 written
-// per value (8 prompts of 2048 tokens into 16 layers: 143 us for 647 MB, 4.5 TB/s; reading the
-// rows a second time, for the codes, took 150).  A decode step's rows are one chain of
+// per value (8 prompts of 2048 tokens into 16 layers: 133 us for 647 MB, 4.9 TB/s; reading the
+// rows a second time, for the codes, took 150, and the largest value in fp32 146).  A decode step's rows are one chain of
 // loads, about 5 us.
 template <int CACHE, bool BF16, int UNIT>
 __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(QuantTables qt, RowTables st, QuantGeom g,
@@ -125,14 +140,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(Qua
   auto read = [&](int i) __attribute__((always_inline)) {
     return *reinterpret_cast<const w4*>(src + ((i >> vs) * a.src_stride + (i & vmask) * 8) * 2);
   };
-  auto largest = [](w4 v) __attribute__((always_inline)) {
-    float f[8], m = 0.f;
-    to_floats<BF16>(v, f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
-    return m;
-  };
-  float top = 0.f;
+  u2 most = u2{0, 0};
   w4 held[kHeld];
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) {
@@ -140,8 +148,10 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(Qua
     if (t + k * UNIT < nvec) held[k] = read(t + k * UNIT);
   }
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k) top = fmaxf(top, largest(held[k]));
-  for (int i = t + kHeld * UNIT; i < nvec; i += UNIT) top = fmaxf(top, largest(read(i)));
+  for (int k = 0; k < kHeld; ++k) most = largest<BF16>(most, held[k]);
+  for (int i = t + kHeld * UNIT; i < nvec; i += UNIT) most = largest<BF16>(most, read(i));
+  const uint32_t bits = max(most[0], most[1]);
+  float top = BF16 ? __uint_as_float(bits << 16) : float(__builtin_bit_cast(_Float16, uint16_t(bits)));
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
   if (UNIT > 64) {
