@@ -30,17 +30,17 @@ namespace {
 template <int BYTES>
 __device__ __forceinline__ void load_words(const char* p, uint32_t* out) {
   if constexpr (BYTES == 16) {
-    const w4 v = __builtin_nontemporal_load(reinterpret_cast<const w4*>(p));
+    const w4 v = *reinterpret_cast<const w4*>(p);
     out[0] = v[0];
     out[1] = v[1];
     out[2] = v[2];
     out[3] = v[3];
   } else if constexpr (BYTES == 8) {
-    const w2 v = __builtin_nontemporal_load(reinterpret_cast<const w2*>(p));
+    const w2 v = *reinterpret_cast<const w2*>(p);
     out[0] = v[0];
     out[1] = v[1];
   } else {
-    out[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+    out[0] = *reinterpret_cast<const uint32_t*>(p);
   }
 }
 
