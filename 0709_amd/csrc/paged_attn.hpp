@@ -333,8 +333,8 @@ struct Pages {
 
 // Joins the splits of a row block: 16 lanes per row, each over D / 16 dims, four rows a
 // wave.  Bound by the chain from the metadata to the partial states, which is walked once a
-// wave: 9.2 us over two chunks of 512 tokens and 32 heads in two splits (24.6 us with one row a
-// wave), 4 to 5 us over one token's rows.
+// wave: 9.3 us over two chunks of 512 tokens and 32 heads in two splits (24.6 us with one row a
+// wave), 4 to 6 us over one token's rows.
 template <int D>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(PagedAttnArgs a) {
   constexpr int DL = D / 16;

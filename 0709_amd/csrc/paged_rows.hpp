@@ -13,8 +13,8 @@
 // exponential counting for four) beside the matrix instructions, which two waves of a SIMD
 // overlap in part.  Four waves on 128 rows, two such workgroups to a CU, or tiles of 32 keys
 // took 3 to 10 % longer: each wave then has more of the staging to do, or meets more barriers.
-// 143 us (460 TFLOP/s) for two chunks of 512 tokens over up to 5464 keys with a distance
-// bias; 74 us (330 TFLOP/s) for four trees of 200 nodes over an int8 cache.
+// 146 us (450 TFLOP/s) for two chunks of 512 tokens over up to 5464 keys with a distance
+// bias; 75 us (320 TFLOP/s) for four trees of 200 nodes over an int8 cache.
 #pragma once
 
 #include "paged_attn.hpp"

@@ -11,12 +11,12 @@
 // c * D/16 .., loads that piece of the rows of its keys, and byte permutes put pairs of
 // keys together.
 //
-// One token: bound by HBM, 99 us for 497 MB (5.0 TB/s) over 32 requests of up to 16384 keys
-// in e4m3; 54 us for 226 MB (4.2 TB/s) over 24 capped requests in bf16 at head_dim 64.  A CU
+// One token: bound by HBM, 98 us for 497 MB (5.1 TB/s) over 32 requests of up to 16384 keys
+// in e4m3; 52 us for 226 MB (4.3 TB/s) over 24 capped requests in bf16 at head_dim 64.  A CU
 // takes in about 50 bytes a ns however many of its waves ask, so few requests want their
 // keys on more CUs: 1024 bf16 keys of 8 heads take 14.0 us whole and 10.1 in six splits.
 // Eight waves a workgroup were 2 % slower there and 20 % where requests are many (their
-// starts and ends overlap less).  Several rows: 31 us for a tree of 36 nodes over 16384 keys
+// starts and ends overlap less).  Several rows: 30 us for a tree of 36 nodes over 16384 keys
 // (144 rows, three blocks), 1.6 to 2.5 us a step of 32 keys, bound by the conversions,
 // permutes and softmax of one wave a SIMD in turn with its matrix instructions; eight waves
 // did not help there either (34.7 against 34.0 us with the join).

@@ -89,9 +89,9 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
 // threads: the rows are read once, into registers (kHeld vectors of 8 values a
 // thread; what a large page holds beyond that is read twice), their largest value
 // gives the scale, and the codes follow.  Bound by the bytes: 2 read and 1 written
-// per value (8 prompts of 2048 tokens into 16 layers: 133 us for 647 MB, 4.9 TB/s; reading the
-// rows a second time, for the codes, took 150, and the largest value in fp32 146).  A decode step's rows are one chain of
-// loads, about 5 us.
+// per value: 128 us for 647 MB, 5.1 TB/s, for 8 prompts of 2048 tokens into 16 layers.  In
+// replays of a graph 133; reading the rows a second time, for the codes, took 150 there, the
+// largest value in fp32 146.  A decode step's rows are one chain of loads, about 5 us.
 template <int CACHE, bool BF16, int UNIT>
 __global__ __launch_bounds__(kAppendThreads) void kv_append_quantized_kernel(QuantTables qt, RowTables st, QuantGeom g,
                                                                              Appends a) {
